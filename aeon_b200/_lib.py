@@ -11,7 +11,9 @@ LIB_PATH = os.path.join(HERE, "libaeon_b200.so")
 
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_DECODE, ERR_IO, END = 0, -1, -2, -3, -4, -5, 1
 
-U8, I8, I16, U16, I32, F32, F64 = range(7)
+U8, I8, I16, U16, I32, F32, F64, F16, BF16 = range(9)
+CODE_INT8, CODE_E4M3 = 0, 1
+DISTILL_MAX_ENTRIES = 256
 INTERP_NEAREST, INTERP_LINEAR, INTERP_CUBIC, INTERP_AREA, INTERP_LANCZOS4 = 0, 1, 2, 3, 4
 
 
@@ -114,6 +116,26 @@ class SpecgramConfig(C.Structure):
                 ("num_cepstra", C.c_int32), ("reserved0", C.c_int32)]
 
 
+class CacheDesc(C.Structure):
+    _fields_ = [
+        ("codes", C.c_void_p), ("scales", C.c_void_p), ("pages", C.c_int64), ("page_tokens", C.c_int32), ("heads", C.c_int32),
+        ("dim", C.c_int32), ("code", C.c_int32), ("table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int32),
+        ("seqs", C.c_int32), ("tokens", C.c_int32), ("dtype", C.c_int32), ("start", C.c_void_p), ("length", C.c_void_p),
+        ("rows", C.c_void_p), ("row_stride_seq", C.c_int64), ("row_stride_token", C.c_int64), ("row_stride_head", C.c_int64),
+        ("values", C.c_void_p), ("value_stride_seq", C.c_int64), ("value_stride_token", C.c_int64),
+        ("value_stride_head", C.c_int64), ("status", C.c_void_p),
+    ]
+
+
+class DistillDesc(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int32), ("dtype", C.c_int32),
+        ("ids", C.c_void_p), ("teacher", C.c_void_p), ("entry_stride", C.c_int64), ("k", C.c_int32), ("temperature", C.c_float),
+        ("weights", C.c_void_p), ("loss", C.c_void_p), ("lse", C.c_void_p), ("grad", C.c_void_p), ("grad_stride", C.c_int64),
+        ("upstream", C.c_void_p), ("grad_scale", C.c_float), ("reserved0", C.c_int32),
+    ]
+
+
 class KernelProfile(C.Structure):
     _fields_ = [("launches", C.c_int64), ("ms", C.c_double), ("algorithmic_bytes", C.c_int64)]
 
@@ -144,6 +166,10 @@ PROTOTYPES = {
                                              C.POINTER(C.c_uint8), C.POINTER(EntropyDesc), C.POINTER(C.c_size_t)]),
     "aeonb_specgram_batch": (C.c_int, [C.c_void_p, C.POINTER(SpecgramDesc), C.c_int, C.POINTER(SpecgramConfig)]),
     "aeonb_specgram_bytes": (C.c_int64, [C.POINTER(SpecgramDesc), C.c_int, C.POINTER(SpecgramConfig)]),
+    "aeonb_cache_write": (C.c_int, [C.c_void_p, C.POINTER(CacheDesc)]),
+    "aeonb_cache_read": (C.c_int, [C.c_void_p, C.POINTER(CacheDesc)]),
+    "aeonb_distill_loss": (C.c_int, [C.c_void_p, C.POINTER(DistillDesc)]),
+    "aeonb_distill_grad": (C.c_int, [C.c_void_p, C.POINTER(DistillDesc)]),
     "aeonb_jpeg_parse": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(JpegInfo)]),
     "aeonb_jpeg_entropy_decode": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]),
     "aeonb_jpeg_roi_for_crop": (C.c_int, [C.POINTER(JpegInfo), C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32)]),

@@ -1,6 +1,6 @@
 """Thin python callers of the batch-kernel entry points (device tensors in, device tensors out).
 
-torch is used for device memory only; every computation happens inside libaeon_b200.so.
+torch is used for device memory and streams only; every computation happens inside libaeon_b200.so.
 """
 import ctypes as C
 
@@ -295,3 +295,179 @@ def jpeg_decode_batch(ctx, encoded, pixel_stride=3):
         L.check(ctx.lib.aeonb_orient_batch(ctx.handle, od, len(turned)))
     ctx.synchronize()
     return outs, descs
+
+
+# ---- operators over torch tensors: the feature cache and the distillation loss.  They run on the context's stream; where another
+# stream is current, the context's stream first waits for it and it then waits for the context's, so tensors need no ordering by
+# the caller (and a capture of the current stream takes the call in).  Under `with torch.cuda.stream(ctx.torch_stream)` nothing waits.
+
+_FLOAT_DTYPE = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+
+
+def _on_context(ctx, call, desc):
+    current = torch.cuda.current_stream(ctx.device)
+    apart = current.cuda_stream != ctx.torch_stream.cuda_stream
+    if apart:
+        ctx.torch_stream.wait_stream(current)
+    L.check(call(ctx.handle, C.byref(desc)))
+    if apart:
+        current.wait_stream(ctx.torch_stream)
+
+
+def _device_tensor(ctx, name, t, dtype, shape=None):
+    """Data pointer of a tensor on the context's GPU, or None for None."""
+    if t is None:
+        return None
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError("%s must be a tensor on cuda:%d" % (name, ctx.device))
+    if t.dtype != dtype:
+        raise ValueError("%s must have the type %s, not %s" % (name, dtype, t.dtype))
+    if shape is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise ValueError("%s must be contiguous with the shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _float_type(name, t):
+    if t.dtype not in _FLOAT_DTYPE:
+        raise ValueError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
+    return _FLOAT_DTYPE[t.dtype]
+
+
+class FeatureCache:
+    """Rows of features in 8 bits in pages on the GPU, with a scale for each token and head (aeonb_cache_write / aeonb_cache_read).
+
+    codes: (pages, page_tokens, heads, dim), torch.int8 or torch.float8_e4m3fn; scales: (pages, page_tokens, heads) float32.
+    Token i of sequence s lies in page table[s, i // page_tokens] at place i % page_tokens; `table` is an int32 tensor (seqs, n).
+    `start` and `length` (int32, one per sequence) give the position of a call's first token and the number of its tokens.  A token
+    without a place in the cache is not written, reads as NaN and sets the int32 tensor `status`, where given, to 1."""
+
+    def __init__(self, ctx, codes, scales):
+        if codes.dtype not in (torch.int8, torch.float8_e4m3fn) or codes.dim() != 4:
+            raise ValueError("codes must be a 4-D tensor of int8 or float8_e4m3fn")
+        _device_tensor(ctx, "codes", codes, codes.dtype, codes.shape)
+        _device_tensor(ctx, "scales", scales, torch.float32, codes.shape[:3])
+        self.ctx, self.codes, self.scales = ctx, codes, scales
+        self.pages, self.page_tokens, self.heads, self.dim = codes.shape
+
+    @classmethod
+    def allocate(cls, ctx, pages, page_tokens, heads, dim, code="int8"):
+        if code not in ("int8", "e4m3"):
+            raise ValueError("the code of a cache is 'int8' or 'e4m3', not %r" % (code,))
+        dev = torch.device("cuda", ctx.device)
+        codes = torch.zeros((pages, page_tokens, heads, dim), dtype=torch.int8, device=dev)
+        return cls(ctx, codes if code == "int8" else codes.view(torch.float8_e4m3fn),
+                   torch.zeros((pages, page_tokens, heads), dtype=torch.float32, device=dev))
+
+    def _desc(self, seqs, tokens, table, start, length, status):
+        ctx = self.ctx
+        d = L.CacheDesc()
+        d.codes, d.scales = self.codes.data_ptr(), self.scales.data_ptr()
+        d.pages, d.page_tokens, d.heads, d.dim = self.pages, self.page_tokens, self.heads, self.dim
+        d.code = L.CODE_INT8 if self.codes.dtype == torch.int8 else L.CODE_E4M3
+        if table.dim() != 2 or table.shape[0] != seqs or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("table must be (%d, n) with the pages of a sequence side by side" % seqs)
+        d.table, d.table_stride, d.table_pages = _device_tensor(ctx, "table", table, torch.int32), table.stride(0), table.shape[1]
+        d.seqs, d.tokens = seqs, tokens
+        d.start = _device_tensor(ctx, "start", start, torch.int32, (seqs,))
+        d.length = _device_tensor(ctx, "length", length, torch.int32, (seqs,))
+        if status is not None and status.numel() < 1:
+            raise ValueError("status must hold a word")
+        d.status = _device_tensor(ctx, "status", status, torch.int32)
+        return d
+
+    def _rows(self, name, t):
+        """The tensor as (seqs, tokens, heads, dim)."""
+        if t.dim() == 3 and self.heads == 1:
+            t = t.unsqueeze(2)
+        if t.dim() != 4 or t.shape[2] != self.heads or t.shape[3] != self.dim or (self.dim > 1 and t.stride(3) != 1):
+            raise ValueError("%s must be (seqs, tokens, %d, %d) with the values of a group side by side, not %s"
+                             % (name, self.heads, self.dim, tuple(t.shape)))
+        return t
+
+    def write(self, rows, table, start=None, length=None, values=None, status=None):
+        """Writes `rows` into the cache; with `values` (a tensor like rows, or rows itself) also the values that the codes stand
+        for.  Rows of `values` behind a sequence's length are left as they are."""
+        rows = self._rows("rows", rows)
+        d = self._desc(rows.shape[0], rows.shape[1], table, start, length, status)
+        d.dtype, d.rows = _float_type("rows", rows), _device_tensor(self.ctx, "rows", rows, rows.dtype)
+        d.row_stride_seq, d.row_stride_token, d.row_stride_head = rows.stride()[:3]
+        if values is not None:
+            values = self._rows("values", values)
+            if values.shape != rows.shape:
+                raise ValueError("values must have the shape of rows")
+            d.values = _device_tensor(self.ctx, "values", values, rows.dtype)
+            d.value_stride_seq, d.value_stride_token, d.value_stride_head = values.stride()[:3]
+        _on_context(self.ctx, self.ctx.lib.aeonb_cache_write, d)
+
+    def read(self, table, tokens, start=None, length=None, out=None, dtype=torch.float32, status=None):
+        """The values of `tokens` tokens of each sequence, (seqs, tokens, heads, dim); zeros behind a sequence's length."""
+        if out is None:
+            out = torch.empty((table.shape[0], tokens, self.heads, self.dim), dtype=dtype, device=self.codes.device)
+        rows = self._rows("out", out)
+        if rows.shape[0] != table.shape[0] or rows.shape[1] != tokens:
+            raise ValueError("out must hold %d tokens of %d sequences" % (tokens, table.shape[0]))
+        d = self._desc(rows.shape[0], tokens, table, start, length, status)
+        d.dtype, d.rows = _float_type("out", rows), _device_tensor(self.ctx, "out", rows, rows.dtype)
+        d.row_stride_seq, d.row_stride_token, d.row_stride_head = rows.stride()[:3]
+        _on_context(self.ctx, self.ctx.lib.aeonb_cache_read, d)
+        return out
+
+
+def _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad):
+    if logits.dim() < 2:
+        raise ValueError("logits must be (..., vocab) with at least two dimensions")
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    if ids.shape[:-1] != lead or ids.shape != teacher.shape:
+        raise ValueError("ids and teacher must be (..., k) with the leading dimensions of logits")
+
+    def rows(name, t):
+        try:
+            t = t if t.dim() == 2 else t.view(-1, t.shape[-1])
+        except RuntimeError:
+            raise ValueError("%s must have rows at one stride" % name) from None
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError("the values of a row of %s must lie side by side" % name)
+        return t
+
+    d = L.DistillDesc()
+    d.dtype, d.logits = _float_type("logits", logits), _device_tensor(ctx, "logits", logits, logits.dtype)
+    n = logits.numel() // max(vocab, 1)
+    x = rows("logits", logits) if n else logits
+    d.logits_stride, d.rows, d.vocab, d.k = x.stride(0), n, vocab, ids.shape[-1]
+    ids, teacher = ids.contiguous(), teacher.contiguous()
+    d.ids, d.teacher = _device_tensor(ctx, "ids", ids, torch.int32), _device_tensor(ctx, "teacher", teacher, torch.float32)
+    d.entry_stride, d.temperature = d.k, temperature
+    d.weights = _device_tensor(ctx, "weights", weights, torch.float32, lead)
+    d.upstream, d.grad_scale = _device_tensor(ctx, "upstream", upstream, torch.float32, lead), grad_scale
+    if grad is not None:
+        if grad.shape != logits.shape:
+            raise ValueError("grad must have the shape of logits")
+        d.grad = _device_tensor(ctx, "grad", grad, logits.dtype)
+        d.grad_stride = (rows("grad", grad) if n else grad).stride(0)
+    return d, (ids, teacher)
+
+
+def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, want_grad=True, grad=None):
+    """Loss of each row against a teacher's top logits, its log-sum-exp, and the gradient of
+    grad_scale * sum(upstream * loss) with respect to the logits, in one pass over them (aeonb_distill_loss).
+
+    logits: (..., vocab) float32, float16 or bfloat16; ids (int32, -1 = no entry) and teacher (float32): (..., k), as the
+    "top_logits" etl type delivers them; weights, upstream: (...) float32.  Returns (loss, lse, grad); grad is None without
+    want_grad, and may be given (a tensor like logits, or logits itself).  A training step goes on with logits.backward(grad)."""
+    if want_grad and grad is None:
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad if want_grad else None)
+    both = torch.empty((2,) + tuple(logits.shape[:-1]), dtype=torch.float32, device=logits.device)
+    d.loss, d.lse = both.data_ptr(), both.data_ptr() + 4 * d.rows
+    _on_context(ctx, ctx.lib.aeonb_distill_loss, d)
+    return both[0], both[1], grad if want_grad else None
+
+
+def distill_grad(ctx, logits, ids, teacher, lse, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, grad=None):
+    """The gradient alone, from the lse that distill_loss returned for the same logits and temperature (aeonb_distill_grad)."""
+    if grad is None:
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad)
+    d.lse = _device_tensor(ctx, "lse", lse, torch.float32, logits.shape[:-1])
+    _on_context(ctx, ctx.lib.aeonb_distill_grad, d)
+    return grad

@@ -8,7 +8,8 @@
  *
  * Levels, from the GPU up:
  *   1. batch kernels over device-resident data (aeonb_jpeg_entropy_batch, aeonb_jpeg_backend_batch,
- *      aeonb_orient_batch, aeonb_rotate_batch, aeonb_image_batch, aeonb_specgram_batch): one launch per batch;
+ *      aeonb_orient_batch, aeonb_rotate_batch, aeonb_image_batch, aeonb_specgram_batch, aeonb_cache_write / _read,
+ *      aeonb_distill_loss / _grad): one launch per batch;
  *   2. host helpers: header parsing, the host Huffman decoder (progressive files, or by choice), PNG decoding,
  *      AVI index parsing, augmentation parameter draws;
  *   3. the provider: encoded records in host memory -> augmented batch, i.e. what
@@ -62,7 +63,7 @@ enum aeonb_kernel_kind
     AEONB_KERNEL_JPEG_BACKEND = 1, /* jpeg_backend_kernel */
     AEONB_KERNEL_IMAGE = 2,        /* aug_pack_kernel */
     AEONB_KERNEL_SPECGRAM = 3,     /* specgram_kernel / specgram_generic_kernel */
-    AEONB_KERNEL_OTHER = 4,        /* rotate, orient, resize passes, rcnn labels */
+    AEONB_KERNEL_OTHER = 4,        /* rotate, orient, resize passes, rcnn labels, feature cache, distillation */
     AEONB_KERNEL_KINDS = 5
 };
 typedef struct aeonb_kernel_profile
@@ -90,7 +91,9 @@ enum aeonb_dtype
     AEONB_U16 = 3,
     AEONB_I32 = 4,
     AEONB_F32 = 5,
-    AEONB_F64 = 6
+    AEONB_F64 = 6,
+    AEONB_F16 = 7, /* the 16-bit floats are types of the feature cache and of the distillation loss (1d, 1e) only */
+    AEONB_BF16 = 8
 };
 
 enum aeonb_interp
@@ -321,6 +324,116 @@ typedef struct aeonb_specgram_config
 
 int aeonb_specgram_batch(aeonb_ctx* ctx, const aeonb_specgram_desc* descs, int n, const aeonb_specgram_config* cfg);
 int64_t aeonb_specgram_bytes(const aeonb_specgram_desc* descs, int n, const aeonb_specgram_config* cfg);
+
+/* ------------------------------------------------------------------------------------------------
+ * 1d. Feature cache: rows of features (a spectrogram's frames, say) kept on the device in 8 bits, in pages, and read back.
+ *     No counterpart in the reference, whose cache keeps encoded records in files (src/cache_system.cpp).
+ *
+ *     A sequence is a list of tokens (frames), a token `heads` groups of `dim` values.  The cache holds `pages` pages of
+ *     `page_tokens` tokens; token i of sequence s lies in page table[s * table_stride + i / page_tokens], at place
+ *     i % page_tokens.  Each token and head has a scale of its own:
+ *
+ *         scale = max(max|x| / Q rounded to float, 2^-126),   Q = 127 (AEONB_CODE_INT8) or 448 (AEONB_CODE_E4M3)
+ *         code  = x / scale to the nearest number of the code, ties to the even one (of the exact quotient)
+ *         value = code * scale, rounded to the type of the rows
+ *
+ *     -infinity (the logarithm of an empty mel filter) is kept as a code of its own, -128 or 0xFF, reads back as -infinity
+ *     and does not count in max|x|.  A group that holds a NaN or +infinity gets the scale NaN and reads back as NaN.
+ *
+ *     aeonb_cache_write puts tokens [start[s], start[s] + n) of each sequence, n = min(length[s], tokens), into their pages;
+ *     with `values` it also writes the values the codes stand for (`values` may be `rows` itself with the same strides).
+ *     Rows of `values` behind the n-th are left as they are.  The pages of one call's sequences must differ (two tokens
+ *     written to one place leave either's bytes there, or some of both).
+ *     aeonb_cache_read writes the values of the same tokens to `rows`; rows behind the n-th are filled with zeros, as behind
+ *     the end of a clip in aeonb_specgram_batch.
+ *     A token whose position is negative or behind the table, or whose page lies outside 0..pages-1, is not written, reads
+ *     as NaN, and sets *status to 1 (where a status word is given; it is never cleared).
+ *
+ *     Both run on the context's stream, make no allocation, copy nothing from host memory and can be captured into a
+ *     CUDA graph.  Table, start and length are device memory, so a captured call follows their contents.
+ * ---------------------------------------------------------------------------------------------- */
+
+enum aeonb_cache_code
+{
+    AEONB_CODE_INT8 = 0,
+    AEONB_CODE_E4M3 = 1
+};
+
+typedef struct aeonb_cache_desc
+{
+    /* the cache */
+    void*   codes;          /* device: pages x page_tokens x heads x dim bytes */
+    float*  scales;         /* device: pages x page_tokens x heads */
+    int64_t pages;
+    int32_t page_tokens, heads, dim;
+    int32_t code;           /* aeonb_cache_code */
+    /* the sequences of this call */
+    const int32_t* table;   /* device: page numbers, table_pages for each sequence */
+    int64_t table_stride;   /* entries between sequences */
+    int32_t table_pages;
+    int32_t seqs, tokens;   /* rows are seqs x tokens x heads x dim */
+    int32_t dtype;          /* of rows and values: AEONB_F32, AEONB_F16 or AEONB_BF16 */
+    const int32_t* start;   /* device: position of each sequence's first token; NULL: 0 */
+    const int32_t* length;  /* device: tokens of each sequence (below 0 counts as 0, above `tokens` as `tokens`); NULL: tokens */
+    /* rows: the dim values of a group lie side by side; strides in elements */
+    void*   rows;           /* device: source of a write, destination of a read */
+    int64_t row_stride_seq, row_stride_token, row_stride_head;
+    void*   values;         /* device, aeonb_cache_write only: NULL or where the values go */
+    int64_t value_stride_seq, value_stride_token, value_stride_head;
+    int32_t* status;        /* device: NULL or a word that is set to 1 when a token has no place */
+} aeonb_cache_desc;
+
+int aeonb_cache_write(aeonb_ctx* ctx, const aeonb_cache_desc* desc);
+int aeonb_cache_read(aeonb_ctx* ctx, const aeonb_cache_desc* desc);
+
+/* ------------------------------------------------------------------------------------------------
+ * 1e. Distillation from a teacher's top logits: the loss against what the "top_logits" etl type delivers, and its gradient.
+ *     No counterpart in the reference (its training targets are labels, boxes and anchors).
+ *
+ *     Row r has student logits s[0..vocab), k entries (id, t) with the teacher's largest logits, a weight w and, with the
+ *     temperature T,
+ *
+ *         p    = softmax of t / T over the entries with id >= 0 and t > -infinity
+ *         lse  = log sum_v exp(s[v] / T)
+ *         loss = w T^2 sum_entries p (log p - s[id] / T + lse)
+ *         grad[v] = grad_scale upstream[r] w T (exp(s[v] / T - lse) - sum of p over the entries with id v)
+ *
+ *     An id may occur more than once (its entries add up).  One entry and T = 1 give the cross entropy with a label.
+ *     Rows with w == 0 or without an entry (padding) have loss, lse and gradient 0, and their logits are not read.  A row with
+ *     an id >= vocab, or whose largest logit is not finite, has loss, lse and gradient NaN.
+ *
+ *     aeonb_distill_loss writes loss and lse (either may be NULL) and, where grad is given, the gradient in the same pass.
+ *     aeonb_distill_grad writes the gradient from the lse of an earlier call.  grad may be logits itself, with the same stride.
+ *     Both run on the context's stream, make no allocation, copy nothing from host memory and can be captured into a CUDA
+ *     graph; the result does not depend on the order in which blocks run.
+ * ---------------------------------------------------------------------------------------------- */
+
+#define AEONB_DISTILL_MAX_ENTRIES 256
+
+typedef struct aeonb_distill_desc
+{
+    const void* logits;     /* device: rows x vocab, the values of a row side by side */
+    int64_t logits_stride;  /* elements between rows */
+    int64_t rows;
+    int32_t vocab;
+    int32_t dtype;          /* of logits and grad: AEONB_F32, AEONB_F16 or AEONB_BF16 */
+    const int32_t* ids;     /* device: rows x k, -1 = no entry */
+    const float* teacher;   /* device: rows x k */
+    int64_t entry_stride;   /* elements between the rows of ids and of teacher */
+    int32_t k;              /* 1..AEONB_DISTILL_MAX_ENTRIES */
+    float   temperature;    /* > 0 */
+    const float* weights;   /* device: one per row; NULL: 1 */
+    float*  loss;           /* device: one per row */
+    float*  lse;            /* device: one per row; read by aeonb_distill_grad */
+    void*   grad;           /* device: rows x vocab */
+    int64_t grad_stride;    /* elements between rows */
+    const float* upstream;  /* device: one factor of the gradient per row; NULL: 1 */
+    float   grad_scale;     /* one factor for all */
+    int32_t reserved0;
+} aeonb_distill_desc;
+
+int aeonb_distill_loss(aeonb_ctx* ctx, const aeonb_distill_desc* desc);
+int aeonb_distill_grad(aeonb_ctx* ctx, const aeonb_distill_desc* desc);
 
 /* ------------------------------------------------------------------------------------------------
  * 2. Host helpers
