@@ -183,6 +183,28 @@ namespace aeonb
         shape.shape = {(int64_t)output_count};
     }
 
+    top_logits_config::top_logits_config(json js)
+    {
+        js.erase("type");
+        required(js, "max_positions");
+        required(js, "k");
+        max_positions = get_int(js, "max_positions", 0);
+        k             = get_int(js, "k", 0);
+        vocab         = get_int(js, "vocab", 0);
+        name          = get_string(js, "name", "");
+        verify_config("top_logits", {"max_positions", "k", "vocab", "name"}, js);
+        if (max_positions <= 0 || k <= 0 || k > AEONB_DISTILL_MAX_ENTRIES || vocab < 0)
+            throw invalid_argument("top_logits: max_positions must be positive, k between 1 and 256, vocab not negative");
+        shapes.resize(3);
+        shapes[0].otype = shapes[2].otype = output_type::from_name("int32_t");
+        shapes[1].otype      = output_type::from_name("float");
+        shapes[0].shape      = {max_positions, k};
+        shapes[0].axis_names = {"position", "entry"};
+        shapes[1].shape      = shapes[0].shape;
+        shapes[1].axis_names = shapes[0].axis_names;
+        shapes[2].shape      = {1};
+    }
+
     video_config::video_config(json js)
     {
         if (js.is_null())

@@ -74,6 +74,19 @@ namespace aeonb
         explicit blob_config(json js);
     };
 
+    // What a teacher answered for a record: for each position its largest logits and their ids, the targets of aeonb_distill_loss.
+    // No counterpart in aeon, whose targets are labels, boxes and anchors.
+    struct top_logits_config
+    {
+        int                     max_positions = 0; // positions behind it are cut, as an audio clip's frames are
+        int                     k             = 0; // entries for each position; records may have fewer
+        int                     vocab         = 0; // ids must be below it; 0: any
+        std::string             name;
+        std::vector<shape_type> shapes; // ids, logits, number of positions
+        top_logits_config() = default;
+        explicit top_logits_config(json js);
+    };
+
     struct video_config
     {
         int          max_frame_count = 0;

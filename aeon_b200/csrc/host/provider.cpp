@@ -224,6 +224,14 @@ aeonb_provider::aeonb_provider(aeonb_ctx* c, const json& cfg) : ctx(c)
             st.blob = blob_config(e);
             add(prefixed(st.blob.name, "blob"), st.blob.shape, true);
         }
+        else if (t == "top_logits")
+        {
+            st.kind       = stage_kind::top_logits;
+            st.top_logits = top_logits_config(e);
+            const char* names[3] = {"teacher_ids", "teacher_logits", "teacher_count"};
+            for (int i = 0; i < 3; ++i)
+                add(prefixed(st.top_logits.name, names[i]), st.top_logits.shapes[i], true);
+        }
         else if (t == "video")
         {
             st.kind  = stage_kind::video;

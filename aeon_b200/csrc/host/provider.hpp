@@ -38,6 +38,7 @@ namespace aeonb
         mask, // pixelmask: a one-channel target picture that follows the image's geometry
         label,
         blob, // bytes copied as they are (host only)
+        top_logits, // a teacher's top logits for each position: ids, logits, count (host only)
         video,
         ssd,
         audio,
@@ -52,6 +53,7 @@ namespace aeonb
         image_config image;
         label_config label;
         blob_config  blob;
+        top_logits_config top_logits;
         video_config video;
         ssd_config   ssd;
         audio_config audio;

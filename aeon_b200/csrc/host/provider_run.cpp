@@ -120,6 +120,43 @@ namespace aeonb
             return r;
         }
 
+        // A top_logits record: int32 positions, int32 entries per position, then the ids (int32) and the logits (float) of all
+        // positions, little endian.  Writes up to cfg.max_positions rows of cfg.k entries, -1 and 0 where there is none, and returns
+        // the number of positions written.
+        int32_t load_top_logits(const uint8_t* data, size_t size, const top_logits_config& cfg, int idx, int32_t* ids, float* logits)
+        {
+            const auto bad = [&](const string& what) {
+                std::stringstream ss;
+                ss << "top logits: " << what << ", at idx " << idx;
+                throw std::runtime_error(ss.str());
+            };
+            int32_t head[2] = {0, 0};
+            if (size >= 8)
+                std::memcpy(head, data, 8);
+            if (size < 8 || head[0] < 0 || head[1] < 1 || (uint64_t)head[0] * head[1] != (size - 8) / 8 || (size - 8) % 8)
+                bad("a record of " + std::to_string(size) + " bytes does not hold the positions and entries that it names");
+            if (head[1] > cfg.k)
+                bad(std::to_string(head[1]) + " entries for each position, the configuration has " + std::to_string(cfg.k));
+            const size_t   all = (size_t)head[0] * head[1], k = (size_t)head[1];
+            const int32_t  n   = std::min(head[0], cfg.max_positions);
+            const uint8_t *from_ids = data + 8, *from_logits = data + 8 + all * 4;
+            std::fill(ids, ids + (size_t)cfg.max_positions * cfg.k, -1);
+            for (size_t i = 0; i < (size_t)n; ++i)
+            {
+                int32_t* row = ids + i * cfg.k;
+                std::memcpy(row, from_ids + i * k * 4, k * 4);
+                std::memcpy(logits + i * cfg.k, from_logits + i * k * 4, k * 4);
+                for (size_t j = 0; j < k; ++j)
+                {
+                    if (row[j] < 0)
+                        row[j] = -1;
+                    else if (cfg.vocab && row[j] >= cfg.vocab)
+                        bad("id " + std::to_string(row[j]) + " is not below the vocab of " + std::to_string(cfg.vocab));
+                }
+            }
+            return n;
+        }
+
         const int16_t* wav_samples(const void* data, size_t size, size_t& count)
         {
             // Raw little-endian int16 samples, or a RIFF/WAVE file whose 'data' chunk holds them.
@@ -467,6 +504,9 @@ void aeonb_provider::plan_records(batch_plan& B, const void* const* elems, const
     for (size_t o = 0; o < outputs.size(); ++o)
         if (outputs[o].host_produced && !(outputs[o].anchor_plane && B.anchor_planes_on_device))
             B.out_host[o].assign((size_t)batch_size * outputs[o].shape.byte_size(), 0);
+    for (const stage& sg : stages)
+        if (sg.kind == stage_kind::top_logits) // no entries in the records that a short batch lacks
+            std::fill(B.out_host[sg.first_output].begin(), B.out_host[sg.first_output].end(), (char)-1);
 
     // Parses the headers of one JPEG stream and registers it as a decode job (sizes only; no layout yet).
     auto plan_jpeg = [&](const void* data, size_t size) -> int {
@@ -943,6 +983,17 @@ void aeonb_provider::plan_records(batch_plan& B, const void* const* elems, const
                     throw std::runtime_error(ss.str());
                 }
                 std::memcpy(B.out_host[sg.first_output].data() + (size_t)r * room, data, size);
+                break;
+            }
+            case stage_kind::top_logits:
+            {
+                if (size == 0)
+                    empty("top logits");
+                const size_t P = (size_t)sg.top_logits.max_positions, K = (size_t)sg.top_logits.k;
+                int32_t*     ids    = reinterpret_cast<int32_t*>(B.out_host[sg.first_output].data()) + (size_t)r * P * K;
+                float*       logits = reinterpret_cast<float*>(B.out_host[sg.first_output + 1].data()) + (size_t)r * P * K;
+                int32_t*     count  = reinterpret_cast<int32_t*>(B.out_host[sg.first_output + 2].data()) + r;
+                *count              = load_top_logits(static_cast<const uint8_t*>(data), size, sg.top_logits, r, ids, logits);
                 break;
             }
             case stage_kind::audio:

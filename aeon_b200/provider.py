@@ -34,6 +34,15 @@ def _bytes_offset():
 _BYTES_AT = _bytes_offset()
 
 
+def top_logits_record(ids, logits):
+    """The bytes of a "top_logits" element: what a teacher answered for each position of a record.  ids (int32, -1 = no entry) and
+    logits (float32) are arrays (positions, k)."""
+    ids, logits = np.asarray(ids, "<i4"), np.asarray(logits, "<f4")
+    if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[1] < 1:
+        raise ValueError("ids and logits must be two arrays (positions, k) of one shape")
+    return np.array(ids.shape, "<i4").tobytes() + ids.tobytes() + logits.tobytes()
+
+
 class Provider:
     def __init__(self, ctx, config):
         self.ctx = ctx

@@ -149,3 +149,37 @@ def test_oracle_codes_are_the_nearest():
     assert s[0] == 1.0
     assert q.view(np.int8).tolist() == [[127, 0, 2, 2, 0, -2, 126, -126, -127, -128]]
     assert ocache.decode(q, s, "int8").tolist() == [[127.0, 0.0, 2.0, 2.0, 0.0, -2.0, 126.0, -126.0, -127.0, -np.inf]]
+
+
+def loader_config(**changes):
+    cfg = {"manifest_filename": "m.tsv", "batch_size": 4, "device_output": True, "feature_cache": "int8",
+           "etl": [{"type": "audio", "max_samples": 3200}, {"type": "label"}, {"type": "top_logits", "max_positions": 4, "k": 2}]}
+    cfg.update(changes)
+    return cfg
+
+
+def test_feature_cache_configurations():
+    from aeon_b200 import DataLoader
+    from aeon_b200.dataloader import check_feature_cache
+    assert check_feature_cache(loader_config()) == "int8"
+    assert check_feature_cache(loader_config(feature_cache="e4m3", iteration_mode="ONCE")) == "e4m3"
+    assert check_feature_cache({"etl": [{"type": "image"}], "shuffle_enable": True}) is None
+    for changes, words in [
+            (dict(feature_cache="int4"), "int8"), (dict(feature_cache=True), "int8"), (dict(device_output=False), "device_output"),
+            (dict(batch_major=False), "batch_major"), (dict(iteration_mode="INFINITE"), "ONCE"),
+            (dict(iteration_mode="COUNT", iteration_mode_count=3), "ONCE"), (dict(shuffle_enable=True), "shuffle"),
+            (dict(etl=[{"type": "label"}]), "audio"), (dict(etl=[{"type": "audio"}, {"type": "image"}]), "image"), (dict(etl=[]), "audio")]:
+        with pytest.raises(ValueError, match=words):
+            DataLoader(loader_config(**changes))
+
+
+def test_top_logits_record_bytes():
+    from aeon_b200.provider import top_logits_record
+    got = top_logits_record([[3, -1], [7, 2], [0, 1]], [[0.5, 0], [2, 1], [-1, -2]])
+    assert np.frombuffer(got[:8], "<i4").tolist() == [3, 2]
+    assert np.frombuffer(got[8:32], "<i4").tolist() == [3, -1, 7, 2, 0, 1]
+    assert np.frombuffer(got[32:], "<f4").tolist() == [0.5, 0, 2, 1, -1, -2]
+    assert top_logits_record(np.zeros((0, 3)), np.zeros((0, 3))) == np.array([0, 3], "<i4").tobytes()
+    for ids, logits in (([1, 2], [1, 2]), ([[1, 2]], [[1, 2, 3]]), (np.zeros((2, 0)), np.zeros((2, 0)))):
+        with pytest.raises(ValueError):
+            top_logits_record(ids, logits)
