@@ -123,7 +123,7 @@ class CacheDesc(C.Structure):
         ("seqs", C.c_int32), ("tokens", C.c_int32), ("dtype", C.c_int32), ("start", C.c_void_p), ("length", C.c_void_p),
         ("rows", C.c_void_p), ("row_stride_seq", C.c_int64), ("row_stride_token", C.c_int64), ("row_stride_head", C.c_int64),
         ("values", C.c_void_p), ("value_stride_seq", C.c_int64), ("value_stride_token", C.c_int64),
-        ("value_stride_head", C.c_int64), ("status", C.c_void_p),
+        ("value_stride_head", C.c_int64), ("status", C.c_void_p), ("stream", C.c_void_p),
     ]
 
 
@@ -132,7 +132,7 @@ class DistillDesc(C.Structure):
         ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int32), ("dtype", C.c_int32),
         ("ids", C.c_void_p), ("teacher", C.c_void_p), ("entry_stride", C.c_int64), ("k", C.c_int32), ("temperature", C.c_float),
         ("weights", C.c_void_p), ("loss", C.c_void_p), ("lse", C.c_void_p), ("grad", C.c_void_p), ("grad_stride", C.c_int64),
-        ("upstream", C.c_void_p), ("grad_scale", C.c_float), ("reserved0", C.c_int32),
+        ("upstream", C.c_void_p), ("grad_scale", C.c_float), ("reserved0", C.c_int32), ("stream", C.c_void_p),
     ]
 
 

@@ -56,7 +56,7 @@ namespace aeonb
 
 namespace aeonb
 {
-    launch_timer::launch_timer(aeonb_ctx* c, int kind, int64_t algorithmic_bytes) : ctx(c)
+    launch_timer::launch_timer(aeonb_ctx* c, int kind, int64_t algorithmic_bytes, cudaStream_t s) : ctx(c), stream(s)
     {
         if (!ctx->profiling)
             return;
@@ -71,7 +71,7 @@ namespace aeonb
             else
                 AEONB_CUDA(cudaEventCreate(e));
         }
-        AEONB_CUDA(cudaEventRecord(sp.begin, ctx->stream));
+        AEONB_CUDA(cudaEventRecord(sp.begin, stream));
         ctx->spans.push_back(sp);
         span = (int)ctx->spans.size() - 1;
     }
@@ -79,7 +79,7 @@ namespace aeonb
     launch_timer::~launch_timer()
     {
         if (span >= 0)
-            cudaEventRecord(ctx->spans[span].end, ctx->stream);
+            cudaEventRecord(ctx->spans[span].end, stream);
     }
 }
 
@@ -223,6 +223,7 @@ int aeonb_ctx_profile_read(aeonb_ctx* ctx, aeonb_kernel_profile out[AEONB_KERNEL
         for (const profile_span& sp : ctx->spans)
         {
             float ms = 0;
+            AEONB_CUDA(cudaEventSynchronize(sp.end)); // it may lie on another stream
             AEONB_CUDA(cudaEventElapsedTime(&ms, sp.begin, sp.end));
             aeonb_kernel_profile& t = ctx->totals[sp.kind];
             t.launches++;

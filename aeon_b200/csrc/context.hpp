@@ -128,14 +128,16 @@ struct aeonb_ctx
 namespace aeonb
 {
     // Brackets the launch(es) of one batch call: counts them and, when the context's profile is on, records a timing
-    // event on the context's stream before and after.
+    // event before and after, on the context's stream or the one given.
     struct launch_timer
     {
-        launch_timer(aeonb_ctx* ctx, int kind, int64_t algorithmic_bytes);
+        launch_timer(aeonb_ctx* ctx, int kind, int64_t algorithmic_bytes) : launch_timer(ctx, kind, algorithmic_bytes, ctx->stream) {}
+        launch_timer(aeonb_ctx* ctx, int kind, int64_t algorithmic_bytes, cudaStream_t stream);
         ~launch_timer();
         launch_timer(const launch_timer&) = delete;
-        aeonb_ctx* ctx;
-        int        span = -1;
+        aeonb_ctx*   ctx;
+        cudaStream_t stream;
+        int          span = -1;
     };
 
     // Validates a batch of image descriptors (throws std::invalid_argument / aeonb::error); reports the

@@ -1,11 +1,19 @@
 // Distillation from a teacher's top logits on sm_100a: the loss of each row, its log-sum-exp, and the gradient.
 //
-// A block per row.  One pass over the logits keeps, in each thread, the largest value so far and the sum of exponentials
-// against it (both in 32 bits, the exponentials to the base 2 with log2(e) / T as a factor of the difference, so that rows at the
-// ends of the type's range do not overflow); a second pass writes the gradient.  The entries' own part of the gradient is written after a barrier, by the first thread that holds the id, with
-// the probabilities of all entries of that id added in their order: no atomics, the same bits every time.
+// A row's logits are read from memory once and stay in registers: the largest value, then the sum of exponentials against it
+// (to the base 2, with log2(e) / T as a factor of the difference, so that rows at the ends of the type's range do not
+// overflow), then the gradient, which is written where the row is.  Floor: the bytes of the row in, and out with the gradient.
+//   * up to 128 values: a warp per row, a value per lane and step (rows that short start on no boundary);
+//   * up to 256 vectors of 16 bytes: a warp per row, up to eight vectors per lane;
+//   * longer: one to sixteen blocks of a cluster per row, each up to eight vectors per thread; a block's largest value and sum go
+//     to the others through shared memory, once;
+//   * beyond what sixteen blocks hold (2^16 vectors), the loss: a block per row that reads it twice.
+// Vectors are whole ones that lie on 16 bytes; the up to seven values before the first and behind the last are a thread's each.
+// The teacher's probabilities are formed while the row is on its way.  The entries' own part of the gradient is written behind a barrier, for each id by the first entry that has it, with the probabilities of all entries of
+// that id added in their order: no atomics, the same bits every time.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "float_rows.cuh"
 
@@ -13,175 +21,762 @@ namespace aeonb
 {
     namespace
     {
-        constexpr int   THREADS = 256;
+        constexpr int   THREADS = 256; // of distill_kernel
         constexpr int   ENTRIES = AEONB_DISTILL_MAX_ENTRIES;
         constexpr float LN2     = 0.693147180559945309417f;
+
+        enum distill_mode
+        {
+            LOSS,      // loss and lse
+            LOSS_GRAD, // and the gradient
+            GRAD       // the gradient from the lse
+        };
 
         struct distill_launch
         {
             aeonb_distill_desc d;
-            float              c;      // log2(e) / T
-            float              factor; // T grad_scale
-            float              tt;     // T^2
+            float              c;       // log2(e) / T
+            float              factor;  // T grad_scale
+            float              tt;      // T^2
+            int                blocks;  // of a row
+            int                vectors; // of a row's slice, for each of its blocks
+            bool               together; // the gradient's rows lie in their 16 bytes as the logits' do
+        };
+
+        // 2^x; results below 2^-126 are 0 (a share of the sum that no type of the gradient holds to a useful precision)
+        __device__ __forceinline__ float pow2(float x)
+        {
+            float r;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+            return r;
+        }
+
+        struct add
+        {
+            __device__ float operator()(float a, float b) const { return __fadd_rn(a, b); }
+        };
+        struct larger // a NaN only where both are
+        {
+            __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
         };
 
         template <typename Op>
-        __device__ __forceinline__ float block_reduce(float v, float* shared, Op op)
+        __device__ __forceinline__ float warp_reduce(float v, Op op)
         {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1)
                 v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+            return v;
+        }
+
+        template <typename Op>
+        __device__ __forceinline__ float block_reduce(float v, float* shared, Op op)
+        {
+            v = warp_reduce(v, op);
             __syncthreads();
             if ((threadIdx.x & 31) == 0)
                 shared[threadIdx.x / 32] = v;
             __syncthreads();
             float r = shared[0];
-            for (int i = 1; i < THREADS / 32; ++i)
+            for (int i = 1; i < (int)blockDim.x / 32; ++i)
                 r = op(r, shared[i]);
             return r;
         }
-        struct add
-        {
-            __device__ float operator()(float a, float b) const { return __fadd_rn(a, b); }
-        };
-        struct larger // NaN where one of the two is
-        {
-            __device__ float operator()(float a, float b) const { return a != a || b != b ? __uint_as_float(0x7fffffffu) : fmaxf(a, b); }
-        };
 
-        __device__ __forceinline__ float pow2(float x) { return exp2f(x); }
-
-        template <typename T, bool WITH_LOSS>
-        __global__ void __launch_bounds__(THREADS) distill_kernel(const distill_launch L)
+        // (x - m) c for two values at once
+        __device__ __forceinline__ float2 scaled_difference(float2 x, float2 minus_m, float2 c)
         {
-            __shared__ float shared[THREADS / 32];
-            __shared__ int   ids[ENTRIES];
-            __shared__ float probs[ENTRIES];
-            const aeonb_distill_desc& d   = L.d;
-            const int                 tid = threadIdx.x;
-            const float               nan = __uint_as_float(0x7fffffffu), inf = __uint_as_float(0x7f800000u);
-            for (int64_t row = blockIdx.x; row < d.rows; row += gridDim.x)
+            float2 r;
+            asm("{ .reg .b64 t, u;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %5};\n"
+                "add.rn.f32x2 t, t, u;\n"
+                "mov.b64 u, {%6, %7};\n"
+                "mul.rn.f32x2 t, t, u;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(x.x), "f"(x.y), "f"(minus_m.x), "f"(minus_m.y), "f"(c.x), "f"(c.y));
+            return r;
+        }
+        __device__ __forceinline__ float2 mul2(float2 a, float2 b)
+        {
+            float2 r;
+            asm("{ .reg .b64 t, u;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %5};\n"
+                "mul.rn.f32x2 t, t, u;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+            return r;
+        }
+        __device__ __forceinline__ float2 add2(float2 a, float2 b)
+        {
+            float2 r;
+            asm("{ .reg .b64 t, u;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %5};\n"
+                "add.rn.f32x2 t, t, u;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+            return r;
+        }
+
+        __device__ __forceinline__ float2 unpack(uint32_t w, __half)
+        {
+            return __half22float2(*reinterpret_cast<const __half2*>(&w));
+        }
+        __device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16)
+        {
+            return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        }
+        __device__ __forceinline__ uint32_t pack(float2 v, __half)
+        {
+            const __half2 h = __floats2half2_rn(v.x, v.y);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+        __device__ __forceinline__ uint32_t pack(float2 v, __nv_bfloat16)
+        {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+        __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __half)
+        {
+            const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+        __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b, __nv_bfloat16)
+        {
+            const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+            return *reinterpret_cast<const uint32_t*>(&h);
+        }
+
+        // Sixteen bytes of a row.
+        template <typename T>
+        struct piece
+        {
+            static constexpr int  N    = 16 / sizeof(T);
+            static constexpr bool WIDE = sizeof(T) == 4;
+            uint32_t              w[4];
+            __device__ __forceinline__ void load(const T* p)
             {
-                const T* s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
-                T*       grad = d.grad ? static_cast<T*>(d.grad) + row * d.grad_stride : nullptr;
-                // the entries: thread i has entry i
-                int   id = -1;
-                float t  = -inf;
-                if (tid < d.k)
+                const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
+                w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+            }
+            __device__ __forceinline__ void clear() // -infinity
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = WIDE ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+            }
+            __device__ __forceinline__ float largest(float m) const
+            {
+                if constexpr (WIDE)
+                    return fmaxf(fmaxf(m, fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]))), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+                else
                 {
-                    id = d.ids[row * d.entry_stride + tid];
-                    t  = d.teacher[row * d.entry_stride + tid];
-                    if (id < 0 || t == -inf)
-                    {
-                        id = -1;
-                        t  = -inf;
-                    }
+                    const float2 v = unpack(max2(max2(w[0], w[1], T()), max2(w[2], w[3], T()), T()), T());
+                    return fmaxf(m, fmaxf(v.x, v.y));
                 }
-                __syncthreads();
-                ids[tid]           = id;
-                const bool  beyond = __syncthreads_or(id >= d.vocab);
-                const float w      = d.weights ? d.weights[row] : 1.0f;
-                const float tmax   = block_reduce(t, shared, larger());
-                if (w == 0.0f || tmax == -inf)
+            }
+            __device__ __forceinline__ float2 pair(int i) const
+            {
+                if constexpr (WIDE)
+                    return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+                else
+                    return unpack(w[i], T());
+            }
+            __device__ __forceinline__ float2 sum(float2 z, float m, float c) const
+            {
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i)
                 {
-                    if (WITH_LOSS && tid == 0)
-                    {
-                        if (d.loss)
-                            d.loss[row] = 0.0f;
-                        if (d.lse)
-                            d.lse[row] = 0.0f;
-                    }
-                    if (grad)
-                        for (int64_t v = tid; v < d.vocab; v += THREADS)
-                            grad[v] = from_float<T>(0.0f);
-                    continue;
+                    const float2 x = scaled_difference(pair(i), make_float2(-m, -m), make_float2(c, c));
+                    z              = add2(z, make_float2(pow2(x.x), pow2(x.y)));
                 }
-                const float e    = id >= 0 ? pow2(__fmul_rn(__fsub_rn(t, tmax), L.c)) : 0.0f;
-                const float esum = block_reduce(e, shared, add());
-                const float p    = __fdiv_rn(e, esum);
-                const float sid  = id >= 0 && !beyond ? to_float(s[id]) : 0.0f;
-                probs[tid]       = p;
+                return z;
+            }
+            __device__ __forceinline__ uint4 gradient(float m, float c, float f) const
+            {
+                uint32_t g[4];
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i)
+                {
+                    const float2 x = scaled_difference(pair(i), make_float2(-m, -m), make_float2(c, c));
+                    const float2 v = mul2(make_float2(pow2(x.x), pow2(x.y)), make_float2(f, f));
+                    if constexpr (WIDE)
+                        g[2 * i] = __float_as_uint(v.x), g[2 * i + 1] = __float_as_uint(v.y);
+                    else
+                        g[i] = pack(v, T());
+                }
+                return make_uint4(g[0], g[1], g[2], g[3]);
+            }
+        };
 
-                float top, sum = 1.0f; // the largest logit (or lse times T), and the sum of exponentials against it
-                float correct = 1.0f;  // factor that makes up for the rounding of lse times T
-                bool  bad = beyond || !(tmax < inf);
-                if (WITH_LOSS)
+        // Writes a piece of the gradient, value by value where it does not lie on 16 bytes.
+        template <typename T>
+        __device__ __forceinline__ void store_piece(T* to, const uint4& q, bool whole)
+        {
+            if (whole)
+            {
+                __stcs(reinterpret_cast<uint4*>(to), q);
+                return;
+            }
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < piece<T>::N; ++i)
+                if constexpr (sizeof(T) == 4)
+                    reinterpret_cast<uint32_t*>(to)[i] = w[i];
+                else
+                    reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+
+        // How a row lies in its 16-byte vectors: `head` values before the first whole one, `n` whole ones, `tail` values.
+        template <typename T>
+        struct cut
+        {
+            int head, n, tail;
+            __device__ __forceinline__ cut(const T* s, int vocab)
+            {
+                head = min((int)((0u - (uint32_t)(uintptr_t)s) & 15u) / (int)sizeof(T), vocab);
+                n    = (vocab - head) / piece<T>::N;
+                tail = vocab - head - n * piece<T>::N;
+            }
+            // the value outside whole vectors that thread i takes (16 threads take one each), -1: none
+            __device__ __forceinline__ int loose(int i, bool first, bool last) const
+            {
+                if (i < 8)
+                    return first && i < head ? i : -1;
+                return last && i - 8 < tail ? head + n * piece<T>::N + i - 8 : -1;
+            }
+        };
+
+        // ---- a cluster's barrier, and a store into another of its blocks' shared memory
+        __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+        __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+        __device__ __forceinline__ void cluster_store(float2* p, uint32_t rank, float2 v)
+        {
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.x), "f"(v.y) : "memory");
+        }
+
+        // The entries of a row, in shared memory.
+        struct entries
+        {
+            int   id[ENTRIES];    // -1: none
+            float p[ENTRIES];     // teacher's probability
+            float t[ENTRIES];     // (t - largest t) c
+            float s[ENTRIES];     // the student's logit at id
+        };
+
+        // An entry: its id (-1 where it does not count) and the teacher's logit; true where the row is NaN for it.
+        __device__ __forceinline__ bool read_entry(const aeonb_distill_desc& d, int64_t row, int k, int& id, float& t)
+        {
+            const float ninf = __uint_as_float(0xff800000u);
+            id = d.ids[row * d.entry_stride + k];
+            t  = d.teacher[row * d.entry_stride + k];
+            if (id < 0 || t == ninf)
+                id = -1, t = ninf;
+            return id >= d.vocab || t != t;
+        }
+
+        // A warp reads a row's entries and forms their probabilities; returns the log2 of their sum.  found: whether there are any;
+        // bad: an id outside the vocabulary, or teacher's logits without a finite largest one.
+        template <typename T>
+        __device__ __forceinline__ float read_entries(const distill_launch& L, int64_t row, const T* s, entries& e, bool& found, bool& bad)
+        {
+            const aeonb_distill_desc& d    = L.d;
+            const int                 lane = threadIdx.x & 31;
+            const float               ninf = __uint_as_float(0xff800000u);
+            float                     top  = ninf;
+            bool                      odd  = false;
+            for (int k = lane; k < d.k; k += 32)
+            {
+                int   id;
+                float t;
+                odd |= read_entry(d, row, k, id, t);
+                e.s[k]  = id >= 0 && id < d.vocab ? to_float(s[id]) : 0.0f;
+                e.id[k] = id;
+                e.t[k]  = t;
+                top     = fmaxf(top, t);
+            }
+            top   = warp_reduce(top, larger());
+            odd   = __any_sync(0xffffffffu, odd);
+            found = odd || top != ninf;
+            bad   = odd || !(top < __uint_as_float(0x7f800000u));
+            float sum = 0.0f;
+            for (int k = lane; k < d.k; k += 32)
+            {
+                const float t = __fmul_rn(__fsub_rn(e.t[k], top), L.c);
+                const float p = e.id[k] >= 0 ? pow2(t) : 0.0f;
+                e.t[k]        = t;
+                e.p[k]        = p;
+                sum           = __fadd_rn(sum, p);
+            }
+            sum = warp_reduce(sum, add());
+            for (int k = lane; k < d.k; k += 32)
+                e.p[k] = __fdiv_rn(e.p[k], sum);
+            return log2f(sum);
+        }
+
+        // The loss of a row, by the warp that has read its entries.
+        __device__ __forceinline__ float entries_loss(const distill_launch& L, const entries& e, float esum2, float top, float zsum2, float w)
+        {
+            float term = 0.0f; // p (log p - s / T + lse), to the base 2
+            for (int k = threadIdx.x & 31; k < L.d.k; k += 32)
+                if (e.p[k] > 0.0f)
+                    term = __fadd_rn(term, __fmul_rn(e.p[k], __fadd_rn(__fsub_rn(e.t[k], esum2),
+                                                                       __fadd_rn(zsum2, __fmul_rn(__fsub_rn(top, e.s[k]), L.c)))));
+            return __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(warp_reduce(term, add()), LN2));
+        }
+
+        // The gradient at an entry's id, if it is the first entry that has it; the rest of the row has been written.
+        template <typename T>
+        __device__ __forceinline__ void entry_gradient(const distill_launch& L, const int* ids, const float* p, T* grad, int k, int id, float s,
+                                                       float top, float f, float fq)
+        {
+            float all   = 0.0f;
+            bool  first = true;
+            for (int j = 0; j < L.d.k; ++j)
+                if (ids[j] == id)
                 {
-                    float m = -inf, z = 0.0f;
-                    bool  isnan = false;
-                    if (!bad)
-                        for (int64_t v = tid; v < d.vocab; v += THREADS)
-                        {
-                            const float x = to_float(s[v]);
-                            isnan |= x != x;
-                            if (x > m)
-                            {
-                                z = m == -inf ? 0.0f : __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, x), L.c)));
-                                m = x;
-                            }
-                            if (m > -inf)
-                                z += pow2(__fmul_rn(__fsub_rn(x, m), L.c));
-                        }
-                    const float all = block_reduce(isnan ? nan : m, shared, larger());
-                    bad |= !(fabsf(all) < inf);
-                    top = all;
-                    sum  = block_reduce(m > -inf && !bad ? __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, all), L.c))) : 0.0f, shared, add());
-                    // p (log p - s / T + lse), to the base 2
-                    float term = 0.0f;
-                    const float l2 = log2f(sum);
-                    if (p > 0.0f)
-                    {
-                        const float logp = __fsub_rn(__fmul_rn(__fsub_rn(t, tmax), L.c), log2f(esum));
-                        term             = __fmul_rn(p, __fadd_rn(logp, __fadd_rn(l2, __fmul_rn(__fsub_rn(all, sid), L.c))));
-                    }
-                    const float total = block_reduce(term, shared, add());
-                    if (tid == 0)
-                    {
-                        if (d.loss)
-                            d.loss[row] = bad ? nan : __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(total, LN2));
-                        if (d.lse)
-                            d.lse[row] = bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(l2, LN2));
-                    }
-                    if (!grad)
-                        continue;
+                    first &= j >= k;
+                    all = __fadd_rn(all, p[j]);
+                }
+            if (first)
+                grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(s, top), L.c))), __fmul_rn(f, all)));
+        }
+
+        __device__ __forceinline__ void write_loss(const aeonb_distill_desc& d, int64_t row, float loss, float lse)
+        {
+            if (d.loss)
+                d.loss[row] = loss;
+            if (d.lse)
+                d.lse[row] = lse;
+        }
+
+        // lse times T, which stands for the largest logit where the lse is given, and the factor that makes up for its rounding
+        __device__ __forceinline__ float2 against_lse(const distill_launch& L, float lse)
+        {
+            const float top = __fmul_rn(lse, L.d.temperature);
+            return make_float2(top, pow2(__fmul_rn(-__fmaf_rn(lse, L.d.temperature, -top), L.c)));
+        }
+
+        // Rows of up to 128 values (a value per lane and step) or 256 vectors: a warp each.
+        template <typename T, int MODE, int NT, int NV, bool VECTOR>
+        __global__ void __launch_bounds__(NT) distill_warp_kernel(const distill_launch L)
+        {
+            extern __shared__ __align__(16) unsigned char dynamic[];
+            const aeonb_distill_desc& d    = L.d;
+            const int                 lane = threadIdx.x & 31;
+            const int64_t             row  = (int64_t)blockIdx.x * (NT / 32) + threadIdx.x / 32;
+            const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
+            if (row >= d.rows)
+                return;
+            entries& e    = reinterpret_cast<entries*>(dynamic)[threadIdx.x / 32];
+            const T* s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
+            T*       grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
+
+            const float w   = d.weights ? d.weights[row] : 1.0f;
+            bool        bad = false, found = false;
+            float       esum2 = 0.0f;
+            piece<T>    x[VECTOR ? NV : 1];
+            float       one[VECTOR ? 1 : NV]; // single values
+            const cut<T> c(s, d.vocab);
+            const int   loose = VECTOR ? c.loose(lane, true, lane < 16) : -1;
+            if (w != 0.0f)
+            {
+                if constexpr (VECTOR)
+                {
+                    one[0] = loose >= 0 ? to_float(s[loose]) : -inf;
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (j * 32 + lane < c.n)
+                            x[j].load(s + c.head + (j * 32 + lane) * piece<T>::N);
+                        else
+                            x[j].clear();
                 }
                 else
                 {
-                    const float lse = d.lse[row];
-                    bad |= !(fabsf(lse) < inf);
-                    top     = __fmul_rn(lse, d.temperature);
-                    correct = pow2(__fmul_rn(-__fmaf_rn(lse, d.temperature, -top), L.c));
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        one[j] = j * 32 + lane < d.vocab ? to_float(s[j * 32 + lane]) : -inf;
                 }
-                float f = __fmul_rn(w, L.factor);
-                if (d.upstream)
-                    f = __fmul_rn(f, d.upstream[row]);
-                if (bad)
-                    f = nan;
-                const float fq = WITH_LOSS ? __fdiv_rn(f, sum) : __fmul_rn(f, correct);
-                for (int64_t v = tid; v < d.vocab; v += THREADS)
-                    grad[v] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(to_float(s[v]), top), L.c))));
-                __syncthreads(); // the entries' logits have been read, and the row written
-                if (!bad && id >= 0)
+                esum2 = read_entries(L, row, s, e, found, bad);
+            }
+            if (!found)
+            {
+                if (MODE != GRAD && lane == 0)
+                    write_loss(d, row, 0.0f, 0.0f);
+                if (MODE != LOSS)
+                    for (int i = lane; i < d.vocab; i += 32)
+                        grad[i] = from_float<T>(0.0f);
+                return;
+            }
+            float top, f, fq;
+            if (MODE != GRAD)
+            {
+                float m = -inf;
+#pragma unroll
+                for (int j = 0; j < (VECTOR ? 1 : NV); ++j)
+                    m = fmaxf(m, one[j]);
+                if constexpr (VECTOR)
                 {
-                    float all   = 0.0f;
-                    bool  first = true;
-                    for (int i = 0; i < d.k; ++i)
-                        if (ids[i] == id)
-                        {
-                            first &= i >= tid;
-                            all = __fadd_rn(all, probs[i]);
-                        }
-                    if (first)
-                        grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(sid, top), L.c))), __fmul_rn(f, all)));
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        m = x[j].largest(m);
+                }
+                top = warp_reduce(m, larger());
+                bad |= !(fabsf(top) < inf);
+                float2 z = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < (VECTOR ? 1 : NV); ++j)
+                    z.x = __fadd_rn(z.x, pow2(__fmul_rn(__fsub_rn(one[j], top), L.c)));
+                if constexpr (VECTOR)
+                {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (j * 32 < c.n)
+                            z = x[j].sum(z, top, L.c);
+                }
+                const float sum   = warp_reduce(__fadd_rn(z.x, z.y), add());
+                const float zsum2 = log2f(sum);
+                bad |= sum != sum;
+                const float loss = entries_loss(L, e, esum2, top, zsum2, w);
+                if (lane == 0)
+                    write_loss(d, row, bad ? nan : loss, bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2)));
+                if (MODE == LOSS)
+                    return;
+                f  = __fmul_rn(w, L.factor);
+                fq = sum;
+            }
+            else
+            {
+                const float  lse = d.lse[row];
+                const float2 at  = against_lse(L, lse);
+                bad |= !(fabsf(lse) < inf);
+                f   = __fmul_rn(w, L.factor);
+                top = at.x;
+                fq  = at.y;
+            }
+            if (d.upstream)
+                f = __fmul_rn(f, d.upstream[row]);
+            if (bad)
+                f = nan;
+            fq = MODE == GRAD ? __fmul_rn(f, fq) : __fdiv_rn(f, fq);
+            if constexpr (VECTOR)
+            {
+                if (loose >= 0)
+                    grad[loose] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one[0], top), L.c))));
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (j * 32 + lane < c.n)
+                        store_piece(grad + c.head + (j * 32 + lane) * piece<T>::N, x[j].gradient(top, L.c, fq), L.together);
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (j * 32 + lane < d.vocab)
+                        grad[j * 32 + lane] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one[j], top), L.c))));
+            }
+            __syncwarp();
+            if (!bad)
+                for (int k = lane; k < d.k; k += 32)
+                    if (e.id[k] >= 0)
+                        entry_gradient(L, e.id, e.p, grad, k, e.id[k], e.s[k], top, f, fq);
+        }
+
+        // Longer rows: the blocks of a cluster (LOSS, LOSS_GRAD), or any number of blocks (GRAD), with NV vectors a thread.  Thread k has
+        // entry k; what the warps find of the entries goes through the same two barriers as what they find of the row.
+        template <typename T, int MODE, int NT, int NV>
+        __global__ void __launch_bounds__(NT, 1024 / NT) distill_block_kernel(const distill_launch L)
+        {
+            constexpr int WARPS = NT / 32, EWARPS = ENTRIES / 32;
+            static_assert(NT >= ENTRIES, "a thread per entry");
+            __shared__ float          part_m[WARPS], part_z[WARPS], part_term[EWARPS];
+            __shared__ float2         part_t[EWARPS], theirs[16];
+            __shared__ int            ids[ENTRIES];
+            __shared__ float          probs[ENTRIES];
+            const aeonb_distill_desc& d    = L.d;
+            const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
+            const int64_t             row  = blockIdx.x / (unsigned)L.blocks;
+            const int                 rank = blockIdx.x % (unsigned)L.blocks;
+            const bool                several = MODE != GRAD && L.blocks > 1;
+            const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
+            if (several)
+                cluster_arrive();
+            const T*     s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
+            T*           grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
+            const cut<T> c(s, d.vocab);
+            // this block's vectors
+            const int  begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
+            const bool first = rank == 0, last = rank == L.blocks - 1;
+            const int  loose = c.loose(tid, first, last && tid < 16);
+            const T*   mine  = s + c.head + (begin + tid) * piece<T>::N;
+
+            const float w   = d.weights ? d.weights[row] : 1.0f;
+            float       up  = MODE != LOSS && d.upstream ? d.upstream[row] : 1.0f;
+            const float lse = MODE == GRAD ? d.lse[row] : 0.0f;
+            piece<T>    x[NV];
+            float       one = -inf;
+            int         id  = -1;
+            float       t = -inf, sid = 0.0f;
+            bool        odd = false;
+            if (w != 0.0f)
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (j * NT + tid < n)
+                        x[j].load(mine + j * NT * piece<T>::N);
+                    else
+                        x[j].clear();
+                if (loose >= 0)
+                    one = to_float(s[loose]);
+                if (tid < d.k)
+                {
+                    odd = read_entry(d, row, tid, id, t);
+                    if (id >= 0 && id < d.vocab)
+                        sid = to_float(s[id]);
                 }
             }
+            // ---- the warps' part of the entries and of the row's largest value
+            float ew = 0.0f; // of this entry, against the largest of its warp
+            if (warp * 32 < d.k)
+            {
+                const float tm = warp_reduce(t, larger());
+                ew             = id >= 0 ? pow2(__fmul_rn(__fsub_rn(t, tm), L.c)) : 0.0f;
+                const float es = warp_reduce(ew, add());
+                odd            = __any_sync(0xffffffffu, odd);
+                if (tid < d.k)
+                    ids[tid] = id;
+                if (lane == 0)
+                    part_t[warp] = make_float2(odd ? nan : tm, es);
+                if (tid < d.k)
+                    t = __fmul_rn(__fsub_rn(t, tm), L.c);
+                sid = id >= 0 ? sid : 0.0f;
+            }
+            float m = one;
+            if (MODE != GRAD)
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    m = x[j].largest(m);
+                m = warp_reduce(m, larger());
+                if (lane == 0)
+                    part_m[warp] = m;
+            }
+            __syncthreads();
+            float tmax = -inf;
+            odd        = false;
+            for (int i = 0; i * 32 < d.k; ++i)
+            {
+                odd |= part_t[i].x != part_t[i].x;
+                tmax = fmaxf(tmax, part_t[i].x);
+            }
+            const bool found = odd || tmax != -inf;
+            bool       bad   = odd || !(tmax < inf);
+            float      esum = 0.0f, esum2 = 0.0f;
+            for (int i = 0; i * 32 < d.k; ++i)
+                if (part_t[i].x > -inf)
+                    esum = __fadd_rn(esum, __fmul_rn(part_t[i].y, pow2(__fmul_rn(__fsub_rn(part_t[i].x, tmax), L.c))));
+            float against = 0.0f;
+            if (MODE != GRAD)
+            {
+                m       = warp_reduce(part_m[lane & (WARPS - 1)], larger());
+                against = fabsf(m) < inf ? m : m > 0.0f ? inf : 0.0f; // (a slice may hold nothing but -infinity)
+            }
+            if (warp * 32 < d.k)
+            {
+                const float shift = __fmul_rn(__fsub_rn(part_t[warp].x, tmax), L.c); // of the warp's largest entry
+                const float p     = id >= 0 ? __fdiv_rn(__fmul_rn(ew, pow2(shift)), esum) : 0.0f;
+                if (tid < d.k)
+                    probs[tid] = p;
+                if (MODE != GRAD && first)
+                {
+                    // p (log p - s / T), to the base 2, but for the logarithm of the entries' sum and against this block's largest logit
+                    float term = p > 0.0f ? __fmul_rn(p, __fadd_rn(__fadd_rn(t, shift), __fmul_rn(__fsub_rn(against, sid), L.c))) : 0.0f;
+                    term       = warp_reduce(term, add());
+                    if (lane == 0)
+                        part_term[warp] = term;
+                }
+            }
+            float top, f, fq;
+            if (MODE != GRAD)
+            {
+                float z = 0.0f;
+                if (w != 0.0f)
+                {
+                    float2 zz = make_float2(pow2(__fmul_rn(__fsub_rn(one, against), L.c)), 0.0f);
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (j * NT < n)
+                            zz = x[j].sum(zz, against, L.c);
+                    z = __fadd_rn(zz.x, zz.y);
+                }
+                z = warp_reduce(z, add());
+                if (lane == 0)
+                    part_z[warp] = z;
+                __syncthreads();
+                z   = warp_reduce(lane < WARPS ? part_z[lane] : 0.0f, add());
+                top = m;
+                if (several)
+                {
+                    cluster_wait(); // every block of the cluster has started (it arrived on entry): its memory may be written
+                    if (warp == 0 && lane < L.blocks)
+                        cluster_store(&theirs[rank], lane, make_float2(m, z));
+                    cluster_arrive();
+                    cluster_wait(); // all have written; nothing touches another block's memory afterwards
+                    const float2 o = lane < L.blocks ? theirs[lane] : make_float2(-inf, 0.0f);
+                    top            = warp_reduce(o.x, larger());
+                    z              = o.x == -inf && o.y == o.y ? 0.0f : __fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c)));
+                    z              = warp_reduce(z, add());
+                }
+                bad |= !(fabsf(top) < inf) || z != z;
+                fq = z;
+                if (first && tid == 0 && w != 0.0f && found)
+                {
+                    const float zsum2 = log2f(z);
+                    float       term  = 0.0f;
+                    esum2             = log2f(esum);
+                    for (int i = 0; i * 32 < d.k; ++i)
+                        term = __fadd_rn(term, part_term[i]);
+                    term = __fadd_rn(__fadd_rn(term, __fmul_rn(__fsub_rn(top, against), L.c)), __fsub_rn(zsum2, esum2));
+                    write_loss(d, row, bad ? nan : __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(term, LN2)),
+                               bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2)));
+                }
+            }
+            else
+            {
+                const float2 at = against_lse(L, lse);
+                bad |= !(fabsf(lse) < inf);
+                top = at.x;
+                fq  = at.y;
+            }
+            if (w == 0.0f || !found)
+            {
+                if (MODE != GRAD && first && tid == 0)
+                    write_loss(d, row, 0.0f, 0.0f);
+                if (MODE != LOSS)
+                {
+                    if (loose >= 0)
+                        grad[loose] = from_float<T>(0.0f);
+                    for (int i = tid; i < n; i += NT)
+                        store_piece(grad + c.head + (begin + i) * piece<T>::N, make_uint4(0, 0, 0, 0), L.together);
+                }
+                return;
+            }
+            if (MODE == LOSS)
+                return;
+            f = __fmul_rn(__fmul_rn(w, L.factor), up);
+            if (bad)
+                f = nan;
+            fq = MODE == GRAD ? __fmul_rn(f, fq) : __fdiv_rn(f, fq);
+            if (loose >= 0)
+                grad[loose] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one, top), L.c))));
+            T* to = grad + c.head + (begin + tid) * piece<T>::N;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (j * NT + tid < n)
+                    store_piece(to + j * NT * piece<T>::N, x[j].gradient(top, L.c, fq), L.together);
+            __syncthreads();
+            // ids of this block's values
+            const int from = first ? 0 : c.head + begin * piece<T>::N, end = last ? d.vocab : c.head + (begin + n) * piece<T>::N;
+            if (!bad && id >= from && id < end)
+                entry_gradient(L, ids, probs, grad, tid, id, sid, top, f, fq);
+        }
+
+        // The loss, and the gradient, of rows beyond what a cluster holds: a block per row, which reads it twice.
+        template <typename T>
+        __global__ void __launch_bounds__(THREADS) distill_kernel(const distill_launch L)
+        {
+            __shared__ float          shared[THREADS / 32];
+            __shared__ entries        e;
+            __shared__ float          esum2_;
+            __shared__ int            flags;
+            const aeonb_distill_desc& d    = L.d;
+            const int                 tid  = threadIdx.x;
+            const float               nan  = __uint_as_float(0x7fffffffu), inf = __uint_as_float(0x7f800000u);
+            const int64_t             row  = blockIdx.x;
+            const T*                  s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
+            T*                        grad = d.grad ? static_cast<T*>(d.grad) + row * d.grad_stride : nullptr;
+            const float               w    = d.weights ? d.weights[row] : 1.0f;
+            if (tid < 32)
+            {
+                bool        found = false, bad = false;
+                const float esum2 = w != 0.0f ? read_entries(L, row, s, e, found, bad) : 0.0f;
+                if (tid == 0)
+                {
+                    esum2_ = esum2;
+                    flags  = (found ? 1 : 0) | (bad ? 2 : 0);
+                }
+            }
+            __syncthreads();
+            if (!(flags & 1))
+            {
+                if (tid == 0)
+                {
+                    if (d.loss)
+                        d.loss[row] = 0.0f;
+                    if (d.lse)
+                        d.lse[row] = 0.0f;
+                }
+                if (grad)
+                    for (int64_t v = tid; v < d.vocab; v += THREADS)
+                        grad[v] = from_float<T>(0.0f);
+                return;
+            }
+            float m = -inf, z = 0.0f;
+            for (int64_t v = tid; v < d.vocab; v += THREADS)
+            {
+                const float x = to_float(s[v]);
+                if (x > m)
+                {
+                    z = m == -inf ? z : __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, x), L.c)));
+                    m = x;
+                }
+                if (!(x == -inf)) // a NaN stays in the sum
+                    z = __fadd_rn(z, pow2(__fmul_rn(__fsub_rn(x, m), L.c)));
+            }
+            const float top = block_reduce(m, shared, larger());
+            const float sum = block_reduce(m > -inf && z == z ? __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, top), L.c))) : z, shared, add());
+            const bool  bad = (flags & 2) || !(fabsf(top) < inf) || sum != sum;
+            if (tid < 32)
+            {
+                const float zsum2 = log2f(sum);
+                const float loss  = entries_loss(L, e, esum2_, top, zsum2, w);
+                if (tid == 0)
+                {
+                    if (d.loss)
+                        d.loss[row] = bad ? nan : loss;
+                    if (d.lse)
+                        d.lse[row] = bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2));
+                }
+            }
+            if (!grad)
+                return;
+            float f = __fmul_rn(w, L.factor);
+            if (d.upstream)
+                f = __fmul_rn(f, d.upstream[row]);
+            if (bad)
+                f = nan;
+            const float fq = __fdiv_rn(f, sum);
+            for (int64_t v = tid; v < d.vocab; v += THREADS)
+                grad[v] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(to_float(s[v]), top), L.c))));
+            __syncthreads();
+            if (!bad)
+                for (int k = tid; k < d.k; k += THREADS)
+                    if (e.id[k] >= 0)
+                        entry_gradient(L, e.id, e.p, grad, k, e.id[k], e.s[k], top, f, fq);
         }
 
         void check_distill(const aeonb_distill_desc& d, bool with_loss)
         {
             const int e = float_size(d.dtype);
-            if (d.rows < 0 || d.rows > 0x7fffffff || d.vocab < 1)
-                throw std::invalid_argument("the logits need between 0 and 2^31-1 rows of at least one value");
+            if (d.rows < 0 || d.rows > 0x7fffffff || d.vocab < 1 || d.vocab > 1 << 30)
+                throw std::invalid_argument("the logits need between 0 and 2^31-1 rows of between 1 and 2^30 values");
             if (d.k < 1 || d.k > ENTRIES)
                 throw std::invalid_argument("a row has between 1 and 256 entries");
             if (!(d.temperature > 0.0f) || !std::isfinite(d.temperature) || !std::isfinite(1.4426950408889634 / d.temperature) ||
@@ -204,10 +799,90 @@ namespace aeonb
                 throw std::invalid_argument("a gradient in place of the logits needs their stride");
         }
 
-        template <typename T>
-        void launch_distill(const distill_launch& L, bool with_loss, unsigned blocks, cudaStream_t stream)
+        template <typename T, int MODE, int NT, int NV, bool VECTOR>
+        cudaError_t launch_warps(const distill_launch& L, cudaStream_t stream)
         {
-            with_loss ? distill_kernel<T, true><<<blocks, THREADS, 0, stream>>>(L) : distill_kernel<T, false><<<blocks, THREADS, 0, stream>>>(L);
+            constexpr int ROWS   = NT / 32;
+            const int64_t blocks = (L.d.rows + ROWS - 1) / ROWS;
+            distill_warp_kernel<T, MODE, NT, NV, VECTOR><<<(unsigned)blocks, NT, sizeof(entries) * ROWS, stream>>>(L);
+            return cudaGetLastError();
+        }
+
+        template <typename T, int MODE, int NT, int NV>
+        cudaError_t launch_blocks(const distill_launch& L, cudaStream_t stream)
+        {
+            auto                kernel = distill_block_kernel<T, MODE, NT, NV>;
+            const int64_t       blocks = L.d.rows * L.blocks;
+            cudaLaunchConfig_t  cfg    = {};
+            cudaLaunchAttribute attr   = {};
+            if (blocks > 0x7fffffff)
+                throw error(AEONB_ERR_UNSUPPORTED, "more rows than a launch takes");
+            cfg.gridDim  = dim3((unsigned)blocks);
+            cfg.blockDim = dim3(NT);
+            cfg.stream   = stream;
+            if (MODE != GRAD && L.blocks > 1)
+            {
+                if (L.blocks > 8)
+                {
+                    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+                    if (e != cudaSuccess)
+                        return e;
+                }
+                attr.id               = cudaLaunchAttributeClusterDimension;
+                attr.val.clusterDim.x = L.blocks;
+                attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+                cfg.attrs    = &attr;
+                cfg.numAttrs = 1;
+            }
+            return cudaLaunchKernelEx(&cfg, kernel, L);
+        }
+
+        template <typename T, int MODE>
+        cudaError_t launch_mode(distill_launch& L, cudaStream_t stream)
+        {
+            const int64_t vocab = L.d.vocab, vectors = vocab * (int64_t)sizeof(T) / 16; // whole ones, at most
+            if (vocab <= 32)
+                return launch_warps<T, MODE, 256, 1, false>(L, stream);
+            if (vocab <= 64)
+                return launch_warps<T, MODE, 256, 2, false>(L, stream);
+            if (vocab <= 128)
+                return launch_warps<T, MODE, 256, 4, false>(L, stream);
+            if (vectors <= 32)
+                return launch_warps<T, MODE, 256, 1, true>(L, stream);
+            if (vectors <= 32 * 2)
+                return launch_warps<T, MODE, 256, 2, true>(L, stream);
+            if (vectors <= 32 * 4)
+                return launch_warps<T, MODE, 256, 4, true>(L, stream);
+            if (vectors <= 32 * 8)
+                return launch_warps<T, MODE, 256, 8, true>(L, stream);
+            // blocks of a row: as many as hold it, and more while they do not fill the SMs and have 4 KB each
+            int64_t blocks = 1;
+            while (blocks * 512 * 8 < vectors)
+                blocks *= 2;
+            while (blocks < 8 && L.d.rows * blocks < 148 && vectors / (blocks * 2) >= 256)
+                blocks *= 2;
+            if (MODE != GRAD && blocks > 16)
+            {
+                distill_kernel<T><<<(unsigned)L.d.rows, THREADS, 0, stream>>>(L);
+                return cudaGetLastError();
+            }
+            L.blocks  = (int)blocks;
+            L.vectors = (int)(((vectors + blocks - 1) / blocks + 7) / 8 * 8); // whole lines of 128 bytes
+            if (L.vectors <= 512)
+                return launch_blocks<T, MODE, 256, 2>(L, stream);
+            if (L.vectors <= 1024)
+                return launch_blocks<T, MODE, 256, 4>(L, stream);
+            if (L.vectors <= 2048)
+                return launch_blocks<T, MODE, 512, 4>(L, stream);
+            return launch_blocks<T, MODE, 512, 8>(L, stream);
+        }
+
+        template <typename T>
+        cudaError_t launch_distill(distill_launch& L, bool with_loss, cudaStream_t stream)
+        {
+            if (!with_loss)
+                return launch_mode<T, GRAD>(L, stream);
+            return L.d.grad ? launch_mode<T, LOSS_GRAD>(L, stream) : launch_mode<T, LOSS>(L, stream);
         }
 
         int run_distill(aeonb_ctx* ctx, const aeonb_distill_desc* desc, bool with_loss)
@@ -220,22 +895,25 @@ namespace aeonb
                     return AEONB_OK;
                 device_scope   scope(ctx->device);
                 distill_launch L;
-                L.d      = *desc;
-                L.c      = (float)(1.4426950408889634074 / desc->temperature);
-                L.factor = (float)((double)desc->temperature * desc->grad_scale);
-                L.tt     = (float)((double)desc->temperature * desc->temperature);
-                const int64_t  bytes  = desc->rows * ((int64_t)desc->vocab * float_size(desc->dtype) * (desc->grad ? 2 : 1) + desc->k * 8 + 8);
-                const unsigned blocks = (unsigned)std::min<int64_t>(desc->rows, 1 << 20);
-                launch_timer   timer(ctx, AEONB_KERNEL_OTHER, bytes);
+                const int      e = float_size(desc->dtype);
+                L.d        = *desc;
+                L.c        = (float)(1.4426950408889634074 / desc->temperature);
+                L.factor   = (float)((double)desc->temperature * desc->grad_scale);
+                L.tt       = (float)((double)desc->temperature * desc->temperature);
+                L.together = (((uintptr_t)desc->logits ^ (uintptr_t)desc->grad) & 15) == 0 &&
+                             (desc->rows == 1 || (desc->logits_stride - desc->grad_stride) * e % 16 == 0);
+                const int64_t bytes = desc->rows * ((int64_t)desc->vocab * e * (desc->grad ? 2 : 1) + desc->k * 8 + 8);
+                const cudaStream_t stream = desc->stream ? static_cast<cudaStream_t>(desc->stream) : ctx->stream;
+                launch_timer  timer(ctx, AEONB_KERNEL_OTHER, bytes, stream);
+                cudaError_t   err = cudaSuccess;
                 switch (desc->dtype)
                 {
-                case AEONB_F32: launch_distill<float>(L, with_loss, blocks, ctx->stream); break;
-                case AEONB_F16: launch_distill<__half>(L, with_loss, blocks, ctx->stream); break;
-                case AEONB_BF16: launch_distill<__nv_bfloat16>(L, with_loss, blocks, ctx->stream); break;
+                case AEONB_F32: err = launch_distill<float>(L, with_loss, stream); break;
+                case AEONB_F16: err = launch_distill<__half>(L, with_loss, stream); break;
+                case AEONB_BF16: err = launch_distill<__nv_bfloat16>(L, with_loss, stream); break;
                 }
-                const cudaError_t e = cudaGetLastError();
-                if (e != cudaSuccess)
-                    throw error(AEONB_ERR_CUDA, cuda_message("distillation kernel launch", e));
+                if (err != cudaSuccess)
+                    throw error(AEONB_ERR_CUDA, cuda_message("distillation kernel launch", err));
                 ctx->launches++;
                 return AEONB_OK;
             });

@@ -232,12 +232,13 @@ namespace aeonb
                 const int64_t  groups = (int64_t)d.seqs * d.tokens * d.heads;
                 const unsigned blocks = (unsigned)std::min<int64_t>((groups + 7) / 8, 148 * 64);
                 const int64_t  values = groups * d.dim;
-                launch_timer   timer(ctx, AEONB_KERNEL_OTHER, values * (float_size(d.dtype) * (d.values && write ? 2 : 1) + 1) + groups * 4);
+                const cudaStream_t stream = d.stream ? static_cast<cudaStream_t>(d.stream) : ctx->stream;
+                launch_timer   timer(ctx, AEONB_KERNEL_OTHER, values * (float_size(d.dtype) * (d.values && write ? 2 : 1) + 1) + groups * 4, stream);
                 switch (d.dtype)
                 {
-                case AEONB_F32: launch_cache<float>(d, write, blocks, ctx->stream); break;
-                case AEONB_F16: launch_cache<__half>(d, write, blocks, ctx->stream); break;
-                case AEONB_BF16: launch_cache<__nv_bfloat16>(d, write, blocks, ctx->stream); break;
+                case AEONB_F32: launch_cache<float>(d, write, blocks, stream); break;
+                case AEONB_F16: launch_cache<__half>(d, write, blocks, stream); break;
+                case AEONB_BF16: launch_cache<__nv_bfloat16>(d, write, blocks, stream); break;
                 }
                 const cudaError_t e = cudaGetLastError();
                 if (e != cudaSuccess)

@@ -297,21 +297,15 @@ def jpeg_decode_batch(ctx, encoded, pixel_stride=3):
     return outs, descs
 
 
-# ---- operators over torch tensors: the feature cache and the distillation loss.  They run on the context's stream; where another
-# stream is current, the context's stream first waits for it and it then waits for the context's, so tensors need no ordering by
-# the caller (and a capture of the current stream takes the call in).  Under `with torch.cuda.stream(ctx.torch_stream)` nothing waits.
+# ---- operators over torch tensors: the feature cache and the distillation loss.  They run on the stream that is current on the
+# context's GPU, as torch's own operators do, so tensors need no ordering by the caller and a capture of that stream takes them in.
 
 _FLOAT_DTYPE = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 
 
-def _on_context(ctx, call, desc):
-    current = torch.cuda.current_stream(ctx.device)
-    apart = current.cuda_stream != ctx.torch_stream.cuda_stream
-    if apart:
-        ctx.torch_stream.wait_stream(current)
+def _on_current_stream(ctx, call, desc):
+    desc.stream = torch.cuda.current_stream(ctx.device).cuda_stream or 1  # 1: cudaStreamLegacy, the default stream
     L.check(call(ctx.handle, C.byref(desc)))
-    if apart:
-        current.wait_stream(ctx.torch_stream)
 
 
 def _device_tensor(ctx, name, t, dtype, shape=None):
@@ -397,7 +391,7 @@ class FeatureCache:
                 raise ValueError("values must have the shape of rows")
             d.values = _device_tensor(self.ctx, "values", values, rows.dtype)
             d.value_stride_seq, d.value_stride_token, d.value_stride_head = values.stride()[:3]
-        _on_context(self.ctx, self.ctx.lib.aeonb_cache_write, d)
+        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_write, d)
 
     def read(self, table, tokens, start=None, length=None, out=None, dtype=torch.float32, status=None):
         """The values of `tokens` tokens of each sequence, (seqs, tokens, heads, dim); zeros behind a sequence's length."""
@@ -409,7 +403,7 @@ class FeatureCache:
         d = self._desc(rows.shape[0], tokens, table, start, length, status)
         d.dtype, d.rows = _float_type("out", rows), _device_tensor(self.ctx, "out", rows, rows.dtype)
         d.row_stride_seq, d.row_stride_token, d.row_stride_head = rows.stride()[:3]
-        _on_context(self.ctx, self.ctx.lib.aeonb_cache_read, d)
+        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_read, d)
         return out
 
 
@@ -459,7 +453,7 @@ def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstr
     d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad if want_grad else None)
     both = torch.empty((2,) + tuple(logits.shape[:-1]), dtype=torch.float32, device=logits.device)
     d.loss, d.lse = both.data_ptr(), both.data_ptr() + 4 * d.rows
-    _on_context(ctx, ctx.lib.aeonb_distill_loss, d)
+    _on_current_stream(ctx, ctx.lib.aeonb_distill_loss, d)
     return both[0], both[1], grad if want_grad else None
 
 
@@ -469,5 +463,5 @@ def distill_grad(ctx, logits, ids, teacher, lse, temperature=1.0, weights=None, 
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad)
     d.lse = _device_tensor(ctx, "lse", lse, torch.float32, logits.shape[:-1])
-    _on_context(ctx, ctx.lib.aeonb_distill_grad, d)
+    _on_current_stream(ctx, ctx.lib.aeonb_distill_grad, d)
     return grad

@@ -349,8 +349,8 @@ int64_t aeonb_specgram_bytes(const aeonb_specgram_desc* descs, int n, const aeon
  *     A token whose position is negative or behind the table, or whose page lies outside 0..pages-1, is not written, reads
  *     as NaN, and sets *status to 1 (where a status word is given; it is never cleared).
  *
- *     Both run on the context's stream, make no allocation, copy nothing from host memory and can be captured into a
- *     CUDA graph.  Table, start and length are device memory, so a captured call follows their contents.
+ *     Both run on the context's stream or the one given (cudaStreamLegacy for the default stream), make no allocation, copy
+ *     nothing from host memory and can be captured into a CUDA graph.  Table, start and length are device memory, so a captured call follows their contents.
  * ---------------------------------------------------------------------------------------------- */
 
 enum aeonb_cache_code
@@ -381,6 +381,7 @@ typedef struct aeonb_cache_desc
     void*   values;         /* device, aeonb_cache_write only: NULL or where the values go */
     int64_t value_stride_seq, value_stride_token, value_stride_head;
     int32_t* status;        /* device: NULL or a word that is set to 1 when a token has no place */
+    void*   stream;         /* cudaStream_t of the call; NULL: the context's stream */
 } aeonb_cache_desc;
 
 int aeonb_cache_write(aeonb_ctx* ctx, const aeonb_cache_desc* desc);
@@ -399,13 +400,15 @@ int aeonb_cache_read(aeonb_ctx* ctx, const aeonb_cache_desc* desc);
  *         grad[v] = grad_scale upstream[r] w T (exp(s[v] / T - lse) - sum of p over the entries with id v)
  *
  *     An id may occur more than once (its entries add up).  One entry and T = 1 give the cross entropy with a label.
- *     Rows with w == 0 or without an entry (padding) have loss, lse and gradient 0, and their logits are not read.  A row with
+ *     Rows with w == 0 or without an entry (padding) have loss, lse and gradient 0, whatever their logits hold.  A row with
  *     an id >= vocab, or whose largest logit is not finite, has loss, lse and gradient NaN.
  *
  *     aeonb_distill_loss writes loss and lse (either may be NULL) and, where grad is given, the gradient in the same pass.
  *     aeonb_distill_grad writes the gradient from the lse of an earlier call.  grad may be logits itself, with the same stride.
- *     Both run on the context's stream, make no allocation, copy nothing from host memory and can be captured into a CUDA
- *     graph; the result does not depend on the order in which blocks run.
+ *     A gradient whose rows lie in their 16 bytes as the logits' rows
+ *     do (any with the logits' stride and alignment) is written in whole vectors, another one value by value.
+ *     Both run on the context's stream or the one given (cudaStreamLegacy for the default stream), make no allocation, copy
+ *     nothing from host memory and can be captured into a CUDA graph; the result does not depend on the order in which blocks run.
  * ---------------------------------------------------------------------------------------------- */
 
 #define AEONB_DISTILL_MAX_ENTRIES 256
@@ -415,7 +418,7 @@ typedef struct aeonb_distill_desc
     const void* logits;     /* device: rows x vocab, the values of a row side by side */
     int64_t logits_stride;  /* elements between rows */
     int64_t rows;
-    int32_t vocab;
+    int32_t vocab;          /* 1..2^30 */
     int32_t dtype;          /* of logits and grad: AEONB_F32, AEONB_F16 or AEONB_BF16 */
     const int32_t* ids;     /* device: rows x k, -1 = no entry */
     const float* teacher;   /* device: rows x k */
@@ -430,6 +433,7 @@ typedef struct aeonb_distill_desc
     const float* upstream;  /* device: one factor of the gradient per row; NULL: 1 */
     float   grad_scale;     /* one factor for all */
     int32_t reserved0;
+    void*   stream;         /* cudaStream_t of the call; NULL: the context's stream */
 } aeonb_distill_desc;
 
 int aeonb_distill_loss(aeonb_ctx* ctx, const aeonb_distill_desc* desc);

@@ -7,8 +7,8 @@ Tolerances, from the operations (u = 2^-24, one float32 rounding; all logarithms
   (E + (V / 32 + 64) u) + 2 |lse| u.
 * loss: w T^2 sum p (log p - s / T + lse): each of the terms is off by 4 u times its size (R + log k + |log V|) and by what lse is.
 * gradient: g (q - P): q relative E plus lse's error, P relative (E + (k + 8) u); then half a step of the type, relative to the
-  result, and half its smallest subnormal.  A q below 2^-126 is a float32 subnormal: 2 ulp of it are 2^-148, and the product with
-  g carries them on as |g| 2^-148.
+  result, and half its smallest subnormal.  Exponentials against the row's largest value (or lse) that are below 2^-126 count as 0:
+  the sum is at least 1, so each is off by 2^-126 at most, and the product with g carries that on as |g| 2^-126.
 """
 import ctypes as C
 
@@ -45,7 +45,7 @@ def bounds(x, want, dtype, t, w, factor, k):
     q = np.exp(y - want[1][:, None])
     grad_tol = np.abs(factor)[:, None] * (q * (lse_tol + e + 4 * U)[:, None] * 1.1 + (np.abs(want[2]) / np.maximum(np.abs(factor)[:, None], 1e-300) + q)
                                           * (e[:, None] + (k + 8) * U)) \
-        + np.abs(want[2]) * torch.finfo(TYPES[dtype]).eps / 2 * 1.01 + TINY[dtype] / 2 + np.abs(factor)[:, None] * 2.0 ** -148
+        + np.abs(want[2]) * torch.finfo(TYPES[dtype]).eps / 2 * 1.01 + TINY[dtype] / 2 + np.abs(factor)[:, None] * 2.0 ** -126
     # rows with a NaN among the logits have no tolerance: they are NaN, or exactly 0 where they do not count
     return tuple(np.where(np.isnan(v), 0.0, v) for v in (loss_tol, lse_tol, grad_tol))
 

@@ -37,8 +37,8 @@ def distill_desc(**changes):
 
 def test_descriptor_sizes():
     # natural alignment on x86-64: computed by hand from the header
-    assert C.sizeof(L.CacheDesc) == 160
-    assert C.sizeof(L.DistillDesc) == 120
+    assert C.sizeof(L.CacheDesc) == 168
+    assert C.sizeof(L.DistillDesc) == 128
 
 
 BAD_CACHE = [
@@ -81,7 +81,7 @@ def test_cache_null_and_empty():
 
 
 BAD_DISTILL = [
-    (dict(dtype=L.U8), "type of the rows"), (dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(vocab=0), "rows"),
+    (dict(dtype=L.U8), "type of the rows"), (dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(vocab=0), "rows"), (dict(vocab=(1 << 30) + 1), "rows"),
     (dict(k=0), "entries"), (dict(k=257), "entries"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
     (dict(temperature=float("inf")), "temperature"),
