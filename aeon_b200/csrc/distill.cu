@@ -12,6 +12,7 @@
 // The teacher's probabilities are formed while the row is on its way.  The entries' own part of the gradient is written behind a barrier, for each id by the first entry that has it, with the probabilities of all entries of
 // that id added in their order: no atomics, the same bits every time.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -23,6 +24,7 @@ namespace aeonb
     {
         constexpr int   THREADS = 256; // of distill_kernel
         constexpr int   ENTRIES = AEONB_DISTILL_MAX_ENTRIES;
+        constexpr int   BLOCK_VECTORS = 8; // vectors of 16 bytes that a thread of distill_block_kernel keeps
         constexpr float LN2     = 0.693147180559945309417f;
 
         enum distill_mode
@@ -252,14 +254,46 @@ namespace aeonb
             }
         };
 
-        // ---- a cluster's barrier, and a store into another of its blocks' shared memory
+        __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+        // ---- what the blocks of a cluster tell one another
         __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
         __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-        __device__ __forceinline__ void cluster_store(float2* p, uint32_t rank, float2 v)
+        // Sends v to the same place in another block's shared memory; that block's barrier (at the same place as this one's) counts the
+        // eight bytes.  Unlike a store before the cluster's barrier it does not wait for the gradient's stores under way.
+        __device__ __forceinline__ void cluster_send(float2* p, uint64_t* barrier, uint32_t rank, float2 v)
         {
-            uint32_t to;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-            asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.x), "f"(v.y) : "memory");
+            asm volatile("{ .reg .b32 to, at;\n"
+                         "mapa.shared::cluster.u32 to, %0, %2;\n"
+                         "mapa.shared::cluster.u32 at, %1, %2;\n"
+                         "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [to], {%3, %4}, [at]; }" ::"r"(shared_address(p)),
+                         "r"(shared_address(barrier)), "r"(rank), "f"(v.x), "f"(v.y)
+                         : "memory");
+        }
+        __device__ __forceinline__ void barrier_init(uint64_t* barrier)
+        {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(barrier)) : "memory");
+        }
+        __device__ __forceinline__ void barrier_expect(uint64_t* barrier, uint32_t bytes)
+        {
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(barrier)), "r"(bytes) : "memory");
+        }
+        // Waits until the barrier's phase of the given parity is complete; false when that takes beyond any reason (seconds).
+        __device__ __forceinline__ bool barrier_wait(uint64_t* barrier, uint32_t parity)
+        {
+            for (int i = 0; i < 1 << 20; ++i)
+            {
+                uint32_t done;
+                asm volatile("{ .reg .pred p;\n"
+                             "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                             "selp.u32 %0, 1, 0, p; }"
+                             : "=r"(done)
+                             : "r"(shared_address(barrier)), "r"(parity)
+                             : "memory");
+                if (done)
+                    return true;
+            }
+            return false;
         }
 
         // The entries of a row, in shared memory.
@@ -489,203 +523,318 @@ namespace aeonb
                         entry_gradient(L, e.id, e.p, grad, k, e.id[k], e.s[k], top, f, fq);
         }
 
-        // Longer rows: the blocks of a cluster (LOSS, LOSS_GRAD), or any number of blocks (GRAD), with NV vectors a thread.  Thread k has
-        // entry k; what the warps find of the entries goes through the same two barriers as what they find of the row.
-        template <typename T, int MODE, int NT, int NV>
-        __global__ void __launch_bounds__(NT, 1024 / NT) distill_block_kernel(const distill_launch L)
+        // What thread k knows of a row before it comes to it: its weight and factors, and entry k.
+        struct row_facts
         {
-            constexpr int WARPS = NT / 32, EWARPS = ENTRIES / 32;
-            static_assert(NT >= ENTRIES, "a thread per entry");
-            __shared__ float          part_m[WARPS], part_z[WARPS], part_term[EWARPS];
-            __shared__ float2         part_t[EWARPS], theirs[16];
-            __shared__ int            ids[ENTRIES];
-            __shared__ float          probs[ENTRIES];
+            float w = 0.0f, up = 1.0f, lse = 0.0f;
+            int   id = -1;
+            float t = 0.0f, s = 0.0f;
+            bool  odd = false;
+        };
+
+        // Longer rows: the blocks of a cluster (LOSS, LOSS_GRAD), or any number of blocks (GRAD).  A block keeps its part of a row, up to NV
+        // vectors for each thread, in shared memory, and goes from row to row: each thread copies its vectors of the next row into the
+        // place of those that it has used for the last time, so that memory is never idle.  No other thread touches them.
+        // Thread k has entry k; what the warps find of the entries goes through the same barriers as what they find of the row.
+        template <typename T, int MODE>
+        __global__ void __launch_bounds__(512, MODE == LOSS_GRAD ? 3 : 3) distill_block_kernel(const distill_launch L)
+        {
+            constexpr int NV = BLOCK_VECTORS, CHUNK = 2, CHUNKS = NV / CHUNK, EWARPS = ENTRIES / 32;
+            extern __shared__ __align__(16) unsigned char dynamic[]; // NV x blockDim.x vectors
+            __shared__ float2   part[16], part_t[EWARPS], theirs[2][16];
+            __shared__ float    part_term[EWARPS], probs[ENTRIES], result[4];
+            __shared__ int      flags;
+            __shared__ int      ids_of[2][ENTRIES]; // of rows in turn: the last row's are still read when the next one's are written
+            __shared__ uint64_t arrived[2];
             const aeonb_distill_desc& d    = L.d;
-            const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
-            const int64_t             row  = blockIdx.x / (unsigned)L.blocks;
+            const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31, nt = blockDim.x;
+            const int64_t             step = gridDim.x / (unsigned)L.blocks;
             const int                 rank = blockIdx.x % (unsigned)L.blocks;
-            const bool                several = MODE != GRAD && L.blocks > 1;
+            const bool                several = MODE != GRAD && L.blocks > 1, first = rank == 0, last = rank == L.blocks - 1;
             const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
             if (several)
+            {
+                if (tid == 0)
+                {
+                    barrier_init(&arrived[0]);
+                    barrier_init(&arrived[1]);
+                    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                }
                 cluster_arrive();
-            const T*     s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
-            T*           grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
-            const cut<T> c(s, d.vocab);
-            // this block's vectors
-            const int  begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
-            const bool first = rank == 0, last = rank == L.blocks - 1;
-            const int  loose = c.loose(tid, first, last && tid < 16);
-            const T*   mine  = s + c.head + (begin + tid) * piece<T>::N;
+            }
 
-            const float w   = d.weights ? d.weights[row] : 1.0f;
-            float       up  = MODE != LOSS && d.upstream ? d.upstream[row] : 1.0f;
-            const float lse = MODE == GRAD ? d.lse[row] : 0.0f;
-            piece<T>    x[NV];
-            float       one = -inf;
-            int         id  = -1;
-            float       t = -inf, sid = 0.0f;
-            bool        odd = false;
-            if (w != 0.0f)
-            {
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-                    if (j * NT + tid < n)
-                        x[j].load(mine + j * NT * piece<T>::N);
-                    else
-                        x[j].clear();
-                if (loose >= 0)
-                    one = to_float(s[loose]);
-                if (tid < d.k)
-                {
-                    odd = read_entry(d, row, tid, id, t);
-                    if (id >= 0 && id < d.vocab)
-                        sid = to_float(s[id]);
-                }
-            }
-            // ---- the warps' part of the entries and of the row's largest value
-            float ew = 0.0f; // of this entry, against the largest of its warp
-            if (warp * 32 < d.k)
-            {
-                const float tm = warp_reduce(t, larger());
-                ew             = id >= 0 ? pow2(__fmul_rn(__fsub_rn(t, tm), L.c)) : 0.0f;
-                const float es = warp_reduce(ew, add());
-                odd            = __any_sync(0xffffffffu, odd);
-                if (tid < d.k)
-                    ids[tid] = id;
-                if (lane == 0)
-                    part_t[warp] = make_float2(odd ? nan : tm, es);
-                if (tid < d.k)
-                    t = __fmul_rn(__fsub_rn(t, tm), L.c);
-                sid = id >= 0 ? sid : 0.0f;
-            }
-            float m = one;
-            if (MODE != GRAD)
-            {
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-                    m = x[j].largest(m);
-                m = warp_reduce(m, larger());
-                if (lane == 0)
-                    part_m[warp] = m;
-            }
-            __syncthreads();
-            float tmax = -inf;
-            odd        = false;
-            for (int i = 0; i * 32 < d.k; ++i)
-            {
-                odd |= part_t[i].x != part_t[i].x;
-                tmax = fmaxf(tmax, part_t[i].x);
-            }
-            const bool found = odd || tmax != -inf;
-            bool       bad   = odd || !(tmax < inf);
-            float      esum = 0.0f, esum2 = 0.0f;
-            for (int i = 0; i * 32 < d.k; ++i)
-                if (part_t[i].x > -inf)
-                    esum = __fadd_rn(esum, __fmul_rn(part_t[i].y, pow2(__fmul_rn(__fsub_rn(part_t[i].x, tmax), L.c))));
-            float against = 0.0f;
-            if (MODE != GRAD)
-            {
-                m       = warp_reduce(part_m[lane & (WARPS - 1)], larger());
-                against = fabsf(m) < inf ? m : m > 0.0f ? inf : 0.0f; // (a slice may hold nothing but -infinity)
-            }
-            if (warp * 32 < d.k)
-            {
-                const float shift = __fmul_rn(__fsub_rn(part_t[warp].x, tmax), L.c); // of the warp's largest entry
-                const float p     = id >= 0 ? __fdiv_rn(__fmul_rn(ew, pow2(shift)), esum) : 0.0f;
-                if (tid < d.k)
-                    probs[tid] = p;
-                if (MODE != GRAD && first)
-                {
-                    // p (log p - s / T), to the base 2, but for the logarithm of the entries' sum and against this block's largest logit
-                    float term = p > 0.0f ? __fmul_rn(p, __fadd_rn(__fadd_rn(t, shift), __fmul_rn(__fsub_rn(against, sid), L.c))) : 0.0f;
-                    term       = warp_reduce(term, add());
-                    if (lane == 0)
-                        part_term[warp] = term;
-                }
-            }
-            float top, f, fq;
-            if (MODE != GRAD)
-            {
-                float z = 0.0f;
+            const uint32_t vectors_at = shared_address(dynamic) + tid * 16, vectors_step = nt * 16;
+            const auto     weight = [&](int64_t r) { return r >= d.rows ? 0.0f : d.weights ? __ldg(d.weights + r) : 1.0f; };
+            const auto     facts  = [&](int64_t r, float w) {
+                row_facts a;
+                a.w = w;
                 if (w != 0.0f)
                 {
-                    float2 zz = make_float2(pow2(__fmul_rn(__fsub_rn(one, against), L.c)), 0.0f);
-#pragma unroll
-                    for (int j = 0; j < NV; ++j)
-                        if (j * NT < n)
-                            zz = x[j].sum(zz, against, L.c);
-                    z = __fadd_rn(zz.x, zz.y);
+                    if (MODE != LOSS && d.upstream)
+                        a.up = d.upstream[r];
+                    if (MODE == GRAD)
+                        a.lse = d.lse[r];
+                    if (tid < d.k)
+                        a.odd = read_entry(d, r, tid, a.id, a.t);
                 }
-                z = warp_reduce(z, add());
-                if (lane == 0)
-                    part_z[warp] = z;
-                __syncthreads();
-                z   = warp_reduce(lane < WARPS ? part_z[lane] : 0.0f, add());
-                top = m;
-                if (several)
-                {
-                    cluster_wait(); // every block of the cluster has started (it arrived on entry): its memory may be written
-                    if (warp == 0 && lane < L.blocks)
-                        cluster_store(&theirs[rank], lane, make_float2(m, z));
-                    cluster_arrive();
-                    cluster_wait(); // all have written; nothing touches another block's memory afterwards
-                    const float2 o = lane < L.blocks ? theirs[lane] : make_float2(-inf, 0.0f);
-                    top            = warp_reduce(o.x, larger());
-                    z              = o.x == -inf && o.y == o.y ? 0.0f : __fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c)));
-                    z              = warp_reduce(z, add());
-                }
-                bad |= !(fabsf(top) < inf) || z != z;
-                fq = z;
-                if (first && tid == 0 && w != 0.0f && found)
-                {
-                    const float zsum2 = log2f(z);
-                    float       term  = 0.0f;
-                    esum2             = log2f(esum);
-                    for (int i = 0; i * 32 < d.k; ++i)
-                        term = __fadd_rn(term, part_term[i]);
-                    term = __fadd_rn(__fadd_rn(term, __fmul_rn(__fsub_rn(top, against), L.c)), __fsub_rn(zsum2, esum2));
-                    write_loss(d, row, bad ? nan : __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(term, LN2)),
-                               bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2)));
-                }
-            }
-            else
+                return a;
+            };
+            // this thread's vectors of a row: the first one, and how many lie behind it a block's width apart
+            struct share
             {
-                const float2 at = against_lse(L, lse);
-                bad |= !(fabsf(lse) < inf);
-                top = at.x;
-                fq  = at.y;
-            }
-            if (w == 0.0f || !found)
-            {
-                if (MODE != GRAD && first && tid == 0)
-                    write_loss(d, row, 0.0f, 0.0f);
-                if (MODE != LOSS)
-                {
-                    if (loose >= 0)
-                        grad[loose] = from_float<T>(0.0f);
-                    for (int i = tid; i < n; i += NT)
-                        store_piece(grad + c.head + (begin + i) * piece<T>::N, make_uint4(0, 0, 0, 0), L.together);
-                }
-                return;
-            }
-            if (MODE == LOSS)
-                return;
-            f = __fmul_rn(__fmul_rn(w, L.factor), up);
-            if (bad)
-                f = nan;
-            fq = MODE == GRAD ? __fmul_rn(f, fq) : __fdiv_rn(f, fq);
-            if (loose >= 0)
-                grad[loose] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one, top), L.c))));
-            T* to = grad + c.head + (begin + tid) * piece<T>::N;
+                const T* from;
+                int      n;
+            };
+            const auto share_of = [&](int64_t r, bool any) {
+                const T*     s = static_cast<const T*>(d.logits) + r * d.logits_stride;
+                const cut<T> c(s, d.vocab);
+                const int    begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
+                return share{s + c.head + (begin + tid) * piece<T>::N, any && tid < n ? (n - tid + nt - 1) / nt : 0};
+            };
+            const auto fetch = [&](const share& v, int j) {
+                if (j < v.n)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vectors_at + j * vectors_step),
+                                 "l"(v.from + (int64_t)j * nt * piece<T>::N)
+                                 : "memory");
+            };
+            const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+            const auto vector = [&](piece<T>& x, int j) {
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3])
+                             : "r"(vectors_at + j * vectors_step)
+                             : "memory");
+            };
+
+            int64_t   row = blockIdx.x / (unsigned)L.blocks;
+            row_facts now = facts(row, weight(row)), then;
+            float     w_then = weight(row + step);
+            share     mine   = share_of(row, now.w != 0.0f);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                if (j * NT + tid < n)
-                    store_piece(to + j * NT * piece<T>::N, x[j].gradient(top, L.c, fq), L.together);
-            __syncthreads();
-            // ids of this block's values
-            const int from = first ? 0 : c.head + begin * piece<T>::N, end = last ? d.vocab : c.head + (begin + n) * piece<T>::N;
-            if (!bad && id >= from && id < end)
-                entry_gradient(L, ids, probs, grad, tid, id, sid, top, f, fq);
+            {
+                fetch(mine, j);
+                if (j % CHUNK == CHUNK - 1)
+                    commit();
+            }
+            if (now.id >= 0 && now.id < d.vocab)
+                now.s = to_float(static_cast<const T*>(d.logits)[row * d.logits_stride + now.id]);
+            if (several)
+                cluster_wait(); // every block of the cluster has started and made its barriers: its memory may be written
+            bool lost = false; // a wait for the other blocks has run out: rows are NaN from there on
+            for (int turn = 0; row < d.rows; row += step, ++turn, now = then)
+            {
+                const int    set  = turn & 1;
+                const T*     s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
+                T*           grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
+                const cut<T> c(s, d.vocab);
+                const int    loose = c.loose(tid, first, last && tid < 16);
+                float        one   = now.w != 0.0f && loose >= 0 ? to_float(s[loose]) : -inf;
+                const share  next  = share_of(row + step, w_then != 0.0f);
+                const float  w     = now.w;
+                then               = facts(row + step, w_then);
+                w_then             = weight(row + 2 * step);
+
+                // ---- the warps' part of the entries, and of the row's largest value and sum
+                int*  ids = ids_of[set];
+                float t = now.t, ew = 0.0f; // ew: of this entry, against the largest of its warp
+                if (warp * 32 < d.k)
+                {
+                    const float tm = warp_reduce(now.id >= 0 ? t : -inf, larger());
+                    t              = __fmul_rn(__fsub_rn(t, tm), L.c);
+                    ew             = now.id >= 0 ? pow2(t) : 0.0f;
+                    const float es  = warp_reduce(ew, add());
+                    const bool  odd = __any_sync(0xffffffffu, now.odd);
+                    if (tid < d.k)
+                        ids[tid] = now.id;
+                    if (lane == 0)
+                        part_t[warp] = make_float2(odd ? nan : tm, es);
+                }
+                if (MODE != GRAD)
+                {
+                    // from the lowest finite value on: a row of nothing but -infinity has the sum 0
+                    float  m = fmaxf(one, -3.40282347e38f);
+                    float2 z = make_float2(pow2(__fmul_rn(__fsub_rn(one, m), L.c)), 0.0f);
+#pragma unroll
+                    for (int q = 0; q < CHUNKS; ++q)
+                    {
+                        if (MODE == LOSS)
+                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
+                        else if (q == 0)
+                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
+                        else if (q == 1)
+                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 2) : "memory");
+                        else if (q == 2)
+                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 3) : "memory");
+                        else
+                            asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        piece<T> x[CHUNK];
+                        if (q * CHUNK < mine.n)
+                        {
+                            float higher = m;
+#pragma unroll
+                            for (int i = 0; i < CHUNK; ++i)
+                            {
+                                if (q * CHUNK + i < mine.n)
+                                    vector(x[i], q * CHUNK + i);
+                                else
+                                    x[i].clear();
+                                higher = x[i].largest(higher);
+                            }
+                            const float scale = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
+                            z                 = mul2(z, make_float2(scale, scale));
+                            m                 = higher;
+#pragma unroll
+                            for (int i = 0; i < CHUNK; ++i)
+                                z = x[i].sum(z, m, L.c);
+                        }
+                        if (MODE == LOSS)
+                        {
+#pragma unroll
+                            for (int i = 0; i < CHUNK; ++i)
+                                fetch(next, q * CHUNK + i);
+                            commit();
+                        }
+                    }
+                    const float wm = warp_reduce(m, larger());
+                    const float wz = warp_reduce(__fmul_rn(__fadd_rn(z.x, z.y), pow2(__fmul_rn(__fsub_rn(m, wm), L.c))), add());
+                    if (lane == 0)
+                        part[warp] = make_float2(wm, wz);
+                }
+                __syncthreads();
+                // the next row's logits at its ids
+                if (then.id >= 0 && then.id < d.vocab)
+                    then.s = to_float(s[step * d.logits_stride + then.id]);
+                if (warp == 0)
+                {
+                    const float2 e    = lane * 32 < d.k ? part_t[lane & (EWARPS - 1)] : make_float2(-inf, 0.0f);
+                    const float  tmax = warp_reduce(e.x, larger());
+                    const bool   odd  = __any_sync(0xffffffffu, e.x != e.x);
+                    const float  esum = warp_reduce(e.x > -inf ? __fmul_rn(e.y, pow2(__fmul_rn(__fsub_rn(e.x, tmax), L.c))) : 0.0f, add());
+                    bool         bad  = odd || !(tmax < inf);
+                    float        top = 0.0f, z = 0.0f;
+                    if (MODE != GRAD)
+                    {
+                        float2 o = lane * 32 < nt ? part[lane & 15] : make_float2(-3.40282347e38f, 0.0f);
+                        top      = warp_reduce(o.x, larger());
+                        z        = warp_reduce(__fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c))), add());
+                        if (several)
+                        {
+                            if (lane == 0)
+                                barrier_expect(&arrived[set], L.blocks * 8);
+                            __syncwarp();
+                            if (lane < L.blocks)
+                                cluster_send(&theirs[set][rank], &arrived[set], lane, make_float2(top, z));
+                            lost |= lost || !barrier_wait(&arrived[set], (turn >> 1) & 1);
+                            bad |= lost;
+                            o   = lane < L.blocks ? theirs[set][lane & 15] : make_float2(-3.40282347e38f, 0.0f);
+                            top = warp_reduce(o.x, larger());
+                            z   = warp_reduce(__fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c))), add());
+                        }
+                        bad |= !(fabsf(top) < inf) || !(z > 0.0f);
+                    }
+                    if (lane == 0)
+                    {
+                        result[0] = tmax;
+                        result[1] = esum;
+                        result[2] = top;
+                        result[3] = z;
+                        flags     = (odd || tmax != -inf ? 1 : 0) | (bad ? 2 : 0);
+                    }
+                }
+                __syncthreads();
+                const bool  found = flags & 1;
+                bool        bad   = flags & 2;
+                const float tmax = result[0], esum = result[1];
+                float       top = result[2];
+                const float z   = result[3];
+                if (warp * 32 < d.k)
+                {
+                    const float shift = __fmul_rn(__fsub_rn(part_t[warp].x, tmax), L.c); // of the warp's largest entry
+                    const float p     = now.id >= 0 ? __fdiv_rn(__fmul_rn(ew, pow2(shift)), esum) : 0.0f;
+                    if (tid < d.k)
+                        probs[tid] = p;
+                    if (MODE != GRAD && first)
+                    {
+                        // p (log p - s / T + lse), to the base 2, but for the logarithms of the two sums
+                        float term = p > 0.0f ? __fmul_rn(p, __fadd_rn(__fadd_rn(t, shift), __fmul_rn(__fsub_rn(top, now.s), L.c))) : 0.0f;
+                        term       = warp_reduce(term, add());
+                        if (lane == 0)
+                            part_term[warp] = term;
+                    }
+                }
+                if (MODE != LOSS)
+                {
+                    T*    to = grad + c.head + (min(rank * L.vectors, c.n) + tid) * piece<T>::N;
+                    float f = 0.0f, fq = 0.0f;
+                    if (MODE == GRAD)
+                    {
+                        const float2 at = against_lse(L, now.lse);
+                        bad |= !(fabsf(now.lse) < inf);
+                        top = at.x;
+                        fq  = at.y;
+                    }
+                    if (found)
+                    {
+                        f  = bad ? nan : __fmul_rn(__fmul_rn(w, L.factor), now.up);
+                        fq = MODE == GRAD ? __fmul_rn(f, fq) : __fdiv_rn(f, z);
+                    }
+                    if (loose >= 0)
+                        grad[loose] = from_float<T>(found ? __fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one, top), L.c))) : 0.0f);
+                    const int written = share_of(row, true).n;
+#pragma unroll
+                    for (int q = 0; q < CHUNKS; ++q)
+                    {
+                        if (MODE == GRAD)
+                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
+#pragma unroll
+                        for (int i = 0; i < CHUNK; ++i)
+                        {
+                            const int j = q * CHUNK + i;
+                            if (j < written)
+                            {
+                                uint4 g = make_uint4(0, 0, 0, 0);
+                                if (found)
+                                {
+                                    piece<T> x;
+                                    vector(x, j);
+                                    g = x.gradient(top, L.c, fq);
+                                }
+                                store_piece(to + (int64_t)j * nt * piece<T>::N, g, L.together);
+                            }
+                            fetch(next, j);
+                        }
+                        commit();
+                    }
+                    __syncthreads();
+                    // ids of this block's values
+                    const int begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
+                    const int from = first ? 0 : c.head + begin * piece<T>::N, end = last ? d.vocab : c.head + (begin + n) * piece<T>::N;
+                    if (found && !bad && now.id >= from && now.id < end)
+                        entry_gradient(L, ids, probs, grad, tid, now.id, now.s, top, f, fq);
+                }
+                else
+                    __syncthreads();
+                if (MODE != GRAD && first && tid == 0)
+                {
+                    float loss = 0.0f, lse = 0.0f;
+                    if (found)
+                    {
+                        const float zsum2 = log2f(z);
+                        float       term  = __fsub_rn(zsum2, log2f(esum));
+                        for (int i = 0; i * 32 < d.k; ++i)
+                            term = __fadd_rn(term, part_term[i]);
+                        loss = bad ? nan : __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(term, LN2));
+                        lse  = bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2));
+                    }
+                    write_loss(d, row, loss, lse);
+                }
+                mine = next;
+            }
+            if (several) // nothing is sent to a block that has left
+            {
+                cluster_arrive();
+                cluster_wait();
+            }
         }
 
         // The loss, and the gradient, of rows beyond what a cluster holds: a block per row, which reads it twice.
@@ -808,32 +957,63 @@ namespace aeonb
             return cudaGetLastError();
         }
 
-        template <typename T, int MODE, int NT, int NV>
+        template <typename T, int MODE>
         cudaError_t launch_blocks(const distill_launch& L, cudaStream_t stream)
         {
-            auto                kernel = distill_block_kernel<T, MODE, NT, NV>;
-            const int64_t       blocks = L.d.rows * L.blocks;
+            auto                kernel = distill_block_kernel<T, MODE>;
             cudaLaunchConfig_t  cfg    = {};
             cudaLaunchAttribute attr   = {};
-            if (blocks > 0x7fffffff)
-                throw error(AEONB_ERR_UNSUPPORTED, "more rows than a launch takes");
-            cfg.gridDim  = dim3((unsigned)blocks);
-            cfg.blockDim = dim3(NT);
-            cfg.stream   = stream;
-            if (MODE != GRAD && L.blocks > 1)
+            // a thread for each NV vectors of a block, and for each entry
+            const int warps      = std::min(16, std::max(ENTRIES / 32, (L.vectors + BLOCK_VECTORS * 32 - 1) / (BLOCK_VECTORS * 32)));
+            cfg.blockDim         = dim3(warps * 32);
+            cfg.dynamicSmemBytes = BLOCK_VECTORS * warps * 32 * 16;
+            cfg.stream           = stream;
+            const bool cluster   = MODE != GRAD && L.blocks > 1;
+            if (cluster)
             {
-                if (L.blocks > 8)
-                {
-                    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-                    if (e != cudaSuccess)
-                        return e;
-                }
                 attr.id               = cudaLaunchAttributeClusterDimension;
                 attr.val.clusterDim.x = L.blocks;
                 attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
                 cfg.attrs    = &attr;
                 cfg.numAttrs = 1;
             }
+            // rows at once: the groups of a row's blocks that find room together, asked for once per kernel, size and device
+            static std::atomic<int> room[64][17][5];
+            int                     size = 0; // log2 of the cluster's blocks
+            while (cluster && 1 << size < L.blocks)
+                ++size;
+            int         device = 0, groups = 0;
+            cudaError_t e = cudaGetDevice(&device);
+            if (e != cudaSuccess)
+                return e;
+            if (device < 64)
+                groups = room[device][warps][size].load(std::memory_order_acquire);
+            if (groups == 0)
+            {
+                if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BLOCK_VECTORS * 512 * 16)) != cudaSuccess ||
+                    (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
+                    return e;
+                cfg.gridDim = dim3(cluster ? L.blocks : 1);
+                if (cluster)
+                    e = cudaOccupancyMaxActiveClusters(&groups, kernel, &cfg);
+                else
+                {
+                    int sms = 0;
+                    e       = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&groups, kernel, warps * 32, cfg.dynamicSmemBytes);
+                    if (e == cudaSuccess)
+                        e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+                    groups *= sms;
+                }
+                if (e != cudaSuccess)
+                    return e;
+                if (groups < 1)
+                    return cudaErrorInvalidConfiguration;
+                if (device < 64)
+                    room[device][warps][size].store(groups, std::memory_order_release);
+            }
+            if (!cluster)
+                groups = std::max(1, groups / L.blocks);
+            cfg.gridDim = dim3((unsigned)(std::min<int64_t>(L.d.rows, groups) * L.blocks));
             return cudaLaunchKernelEx(&cfg, kernel, L);
         }
 
@@ -856,8 +1036,9 @@ namespace aeonb
             if (vectors <= 32 * 8)
                 return launch_warps<T, MODE, 256, 8, true>(L, stream);
             // blocks of a row: as many as hold it, and more while they do not fill the SMs and have 4 KB each
-            int64_t blocks = 1;
-            while (blocks * 512 * 8 < vectors)
+            constexpr int most   = BLOCK_VECTORS * 512;
+            int64_t       blocks = 1;
+            while (blocks * most < vectors)
                 blocks *= 2;
             while (blocks < 8 && L.d.rows * blocks < 148 && vectors / (blocks * 2) >= 256)
                 blocks *= 2;
@@ -868,13 +1049,7 @@ namespace aeonb
             }
             L.blocks  = (int)blocks;
             L.vectors = (int)(((vectors + blocks - 1) / blocks + 7) / 8 * 8); // whole lines of 128 bytes
-            if (L.vectors <= 512)
-                return launch_blocks<T, MODE, 256, 2>(L, stream);
-            if (L.vectors <= 1024)
-                return launch_blocks<T, MODE, 256, 4>(L, stream);
-            if (L.vectors <= 2048)
-                return launch_blocks<T, MODE, 512, 4>(L, stream);
-            return launch_blocks<T, MODE, 512, 8>(L, stream);
+            return launch_blocks<T, MODE>(L, stream);
         }
 
         template <typename T>
