@@ -71,6 +71,14 @@ namespace aeonb
             return v;
         }
 
+        // The largest value of a warp, a NaN only where all are (as fmaxf), in one instruction.
+        __device__ __forceinline__ float warp_reduce(float v, larger)
+        {
+            float r;
+            asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+            return r;
+        }
+
         template <typename Op>
         __device__ __forceinline__ float block_reduce(float v, float* shared, Op op)
         {
@@ -383,6 +391,35 @@ namespace aeonb
                 grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(s, top), L.c))), __fmul_rn(f, all)));
         }
 
+        // Whether an id occurs more than once among a row's entries: a warp enters them into a table of twice as many places.
+        __device__ __forceinline__ bool repeats(const int* ids, int* table, int k)
+        {
+            const int lane = threadIdx.x & 31;
+            if (k <= 32)
+            {
+                const int      id   = lane < k ? ids[lane] : -1;
+                const unsigned same = __match_any_sync(0xffffffffu, id); // (all lanes take part)
+                return __any_sync(0xffffffffu, id >= 0 && __popc(same) > 1);
+            }
+            for (int i = lane; i < 2 * ENTRIES; i += 32)
+                table[i] = -1;
+            __syncwarp();
+            bool twice = false;
+            for (int i = lane; i < k; i += 32)
+            {
+                const int id = ids[i];
+                for (uint32_t at = (uint32_t)id * 2654435761u >> 23; id >= 0; at = (at + 1) & (2 * ENTRIES - 1))
+                {
+                    const int there = atomicCAS(&table[at], -1, id); // (which of two equal ones enters does not matter)
+                    twice |= there == id;
+                    if (there == -1 || there == id)
+                        break;
+                }
+            }
+            static_assert(2 * ENTRIES == 1 << (32 - 23), "the hash has as many values as the table places");
+            return __any_sync(0xffffffffu, twice);
+        }
+
         __device__ __forceinline__ void write_loss(const aeonb_distill_desc& d, int64_t row, float loss, float lse)
         {
             if (d.loss)
@@ -523,35 +560,40 @@ namespace aeonb
                         entry_gradient(L, e.id, e.p, grad, k, e.id[k], e.s[k], top, f, fq);
         }
 
-        // What thread k knows of a row before it comes to it: its weight and factors, and entry k.
-        struct row_facts
-        {
-            float w = 0.0f, up = 1.0f, lse = 0.0f;
-            int   id = -1;
-            float t = 0.0f, s = 0.0f;
-            bool  odd = false;
-        };
+        // ---- named barriers of a block: those who wait, and those who only say that they have come
+        __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+        __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
         // Longer rows: the blocks of a cluster (LOSS, LOSS_GRAD), or any number of blocks (GRAD).  A block keeps its part of a row, up to NV
-        // vectors for each thread, in shared memory, and goes from row to row: each thread copies its vectors of the next row into the
-        // place of those that it has used for the last time, so that memory is never idle.  No other thread touches them.
-        // Thread k has entry k; what the warps find of the entries goes through the same barriers as what they find of the row.
-        template <typename T, int MODE>
-        __global__ void __launch_bounds__(512, MODE == LOSS_GRAD ? 3 : 3) distill_block_kernel(const distill_launch L)
+        // vectors for each of NT threads, in shared memory, and goes from row to row: each thread copies its vectors of the next row into
+        // the place of those that it has used for the last time, so that memory is never idle.  No other thread touches them.
+        // The last warp has no vectors.  It reads the entries of the next row while the others work on this one, puts the warps' sums
+        // (and the other blocks') together, hands out what the gradient needs, and writes the entries' own part when the rest is there.
+        // So the others wait once in a row, from their last exponential to the first store.
+        template <typename T, int MODE, int NT>
+        __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : 5) distill_block_kernel(const distill_launch L)
         {
-            constexpr int NV = BLOCK_VECTORS, CHUNK = 2, CHUNKS = NV / CHUNK, EWARPS = ENTRIES / 32;
-            extern __shared__ __align__(16) unsigned char dynamic[]; // NV x blockDim.x vectors
-            __shared__ float2   part[16], part_t[EWARPS], theirs[2][16];
-            __shared__ float    part_term[EWARPS], probs[ENTRIES], result[4];
-            __shared__ int      flags;
-            __shared__ int      ids_of[2][ENTRIES]; // of rows in turn: the last row's are still read when the next one's are written
+            constexpr int NV = BLOCK_VECTORS, CHUNK = 2, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
+            constexpr int SUMS = 1, RESULT = 2, WRITTEN = 3; // barriers
+            static_assert(CHUNKS == 4, "waits for four copies");
+            struct outcome // of a row's sums
+            {
+                float top, fq; // the gradient at v is fq 2^((s[v] - top) c), less the entries' part
+                int   found;   // 0: the row counts for nothing, the gradient is 0
+                int   ahead;   // whether the row that is copied next is needed
+            };
+            extern __shared__ __align__(16) unsigned char dynamic[]; // NV x NT vectors
+            __shared__ float2   part[WARPS], theirs[2][16];
+            __shared__ entries  of_row[2]; // of this row and of the next one
+            __shared__ outcome  result;
+            __shared__ int      table[2 * ENTRIES];
             __shared__ uint64_t arrived[2];
             const aeonb_distill_desc& d    = L.d;
-            const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31, nt = blockDim.x;
+            const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
             const int64_t             step = gridDim.x / (unsigned)L.blocks;
             const int                 rank = blockIdx.x % (unsigned)L.blocks;
             const bool                several = MODE != GRAD && L.blocks > 1, first = rank == 0, last = rank == L.blocks - 1;
-            const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
+            const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu), lowest = -3.40282347e38f;
             if (several)
             {
                 if (tid == 0)
@@ -561,162 +603,241 @@ namespace aeonb
                     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
                 }
                 cluster_arrive();
+                cluster_wait(); // every block of the cluster has started and made its barriers: its memory may be written
             }
+            const auto weight = [&](int64_t r) { return r >= d.rows ? 0.0f : d.weights ? __ldg(d.weights + r) : 1.0f; };
+            int64_t    row    = blockIdx.x / (unsigned)L.blocks;
+            const T*   s      = static_cast<const T*>(d.logits) + row * d.logits_stride;
 
-            const uint32_t vectors_at = shared_address(dynamic) + tid * 16, vectors_step = nt * 16;
-            const auto     weight = [&](int64_t r) { return r >= d.rows ? 0.0f : d.weights ? __ldg(d.weights + r) : 1.0f; };
-            const auto     facts  = [&](int64_t r, float w) {
-                row_facts a;
-                a.w = w;
-                if (w != 0.0f)
+            if (warp < WARPS)
+            {
+                const uint32_t vectors_at = shared_address(dynamic) + tid * 16;
+                // this block's part of a row
+                struct share
                 {
+                    int at;    // this thread's first vector's first value
+                    int left;  // vectors from there on
+                    int loose; // the value outside the vectors that is this thread's; -1: none
+                };
+                const auto share_of = [&](const T* s) {
+                    const cut<T> c(s, d.vocab);
+                    const int    begin = min(rank * L.vectors, c.n);
+                    return share{c.head + (begin + tid) * N, min(L.vectors, c.n - begin) - tid, c.loose(tid, first, last && tid < 16)};
+                };
+                const auto fetch = [&](const T* from, int left, int j) {
+                    if (j * NT < left)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vectors_at + j * NT * 16), "l"(from + j * NT * N) : "memory");
+                };
+                const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+                const auto vector = [&](piece<T>& x, int j) {
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3])
+                                 : "r"(vectors_at + j * NT * 16)
+                                 : "memory");
+                };
+
+                bool  needed = weight(row) != 0.0f, needed_then = MODE == LOSS && weight(row + step) != 0.0f;
+                share mine   = share_of(s);
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                {
+                    fetch(s + mine.at, needed ? mine.left : 0, j);
+                    if (j % CHUNK == CHUNK - 1)
+                        commit();
+                }
+                for (; row < d.rows; row += step)
+                {
+                    const T*    s_then = s + step * d.logits_stride;
+                    const share next   = share_of(s_then);
+                    const float one    = needed && mine.loose >= 0 ? to_float(s[mine.loose]) : -inf;
+                    if (MODE != GRAD)
+                    {
+                        // from the lowest finite value on: a row of nothing but -infinity has the sum 0
+                        const int have = needed ? mine.left : 0, coming = needed_then ? next.left : 0;
+                        float     m    = fmaxf(one, lowest);
+                        float2    z    = make_float2(pow2(__fmul_rn(__fsub_rn(one, m), L.c)), 0.0f);
+#pragma unroll
+                        for (int q = 0; q < CHUNKS; ++q)
+                        {
+                            if (MODE == LOSS || q == 0)
+                                asm volatile("cp.async.wait_group 3;" ::: "memory");
+                            else if (q == 1)
+                                asm volatile("cp.async.wait_group 2;" ::: "memory");
+                            else if (q == 2)
+                                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                            else
+                                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            if (q * CHUNK * NT < have)
+                            {
+                                piece<T> x[CHUNK];
+                                vector(x[0], q * CHUNK);
+                                if ((q * CHUNK + 1) * NT < have)
+                                    vector(x[1], q * CHUNK + 1);
+                                else
+                                    x[1].clear();
+                                const float higher = x[1].largest(x[0].largest(m));
+                                const float scale  = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
+                                m                  = higher;
+                                z                  = x[1].sum(x[0].sum(mul2(z, make_float2(scale, scale)), m, L.c), m, L.c);
+                            }
+                            if (MODE == LOSS)
+                            {
+                                fetch(s_then + next.at, coming, q * CHUNK);
+                                fetch(s_then + next.at, coming, q * CHUNK + 1);
+                                commit();
+                            }
+                        }
+                        const float wm = warp_reduce(m, larger());
+                        const float wz = warp_reduce(__fmul_rn(__fadd_rn(z.x, z.y), pow2(__fmul_rn(__fsub_rn(m, wm), L.c))), add());
+                        if (lane == 0)
+                            part[warp] = make_float2(wm, wz);
+                        bar_arrive(SUMS, ALL);
+                    }
+                    bar_sync(RESULT, ALL);
+                    const outcome o = result;
+                    if (MODE == LOSS)
+                    {
+                        needed      = needed_then;
+                        needed_then = o.ahead;
+                    }
+                    else
+                    {
+                        T*        grad   = static_cast<T*>(d.grad) + row * d.grad_stride;
+                        T*        to     = grad + mine.at;
+                        const int coming = o.ahead ? next.left : 0;
+                        if (mine.loose >= 0)
+                            grad[mine.loose] = from_float<T>(o.found ? __fmul_rn(o.fq, pow2(__fmul_rn(__fsub_rn(one, o.top), L.c))) : 0.0f);
+                        if (o.found && L.together)
+                        {
+#pragma unroll
+                            for (int j = 0; j < NV; ++j)
+                            {
+                                if (MODE == GRAD && j % CHUNK == 0)
+                                    asm volatile("cp.async.wait_group 3;" ::: "memory");
+                                if (j * NT < mine.left)
+                                {
+                                    piece<T> x;
+                                    vector(x, j);
+                                    __stcs(reinterpret_cast<uint4*>(to + j * NT * N), x.gradient(o.top, L.c, o.fq));
+                                }
+                                fetch(s_then + next.at, coming, j);
+                                if (j % CHUNK == CHUNK - 1)
+                                    commit();
+                            }
+                        }
+                        else
+                        {
+                            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+                            for (int j = 0; j < NV; ++j)
+                            {
+                                if (j * NT < mine.left)
+                                {
+                                    uint4 g = make_uint4(0, 0, 0, 0);
+                                    if (o.found)
+                                    {
+                                        piece<T> x;
+                                        vector(x, j);
+                                        g = x.gradient(o.top, L.c, o.fq);
+                                    }
+                                    store_piece(to + j * NT * N, g, L.together);
+                                }
+                                fetch(s_then + next.at, coming, j);
+                            }
+                            for (int q = 0; q < CHUNKS; ++q) // all in the first one: the next row waits for as many as ever
+                                commit();
+                        }
+                        bar_arrive(WRITTEN, ALL);
+                        needed = o.ahead;
+                    }
+                    mine = next;
+                    s    = s_then;
+                }
+            }
+            else
+            {
+                // what this warp knows of a row
+                struct facts
+                {
+                    float w, up, lse;
+                    float esum2;
+                    bool  found, bad;
+                };
+                const auto prepare = [&](int64_t r, float w, const T* s, entries& e) {
+                    facts a{w, 1.0f, 0.0f, 0.0f, false, false};
+                    if (w == 0.0f)
+                        return a;
                     if (MODE != LOSS && d.upstream)
                         a.up = d.upstream[r];
                     if (MODE == GRAD)
                         a.lse = d.lse[r];
-                    if (tid < d.k)
-                        a.odd = read_entry(d, r, tid, a.id, a.t);
-                }
-                return a;
-            };
-            // this thread's vectors of a row: the first one, and how many lie behind it a block's width apart
-            struct share
-            {
-                const T* from;
-                int      n;
-            };
-            const auto share_of = [&](int64_t r, bool any) {
-                const T*     s = static_cast<const T*>(d.logits) + r * d.logits_stride;
-                const cut<T> c(s, d.vocab);
-                const int    begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
-                return share{s + c.head + (begin + tid) * piece<T>::N, any && tid < n ? (n - tid + nt - 1) / nt : 0};
-            };
-            const auto fetch = [&](const share& v, int j) {
-                if (j < v.n)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vectors_at + j * vectors_step),
-                                 "l"(v.from + (int64_t)j * nt * piece<T>::N)
-                                 : "memory");
-            };
-            const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-            const auto vector = [&](piece<T>& x, int j) {
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3])
-                             : "r"(vectors_at + j * vectors_step)
-                             : "memory");
-            };
-
-            int64_t   row = blockIdx.x / (unsigned)L.blocks;
-            row_facts now = facts(row, weight(row)), then;
-            float     w_then = weight(row + step);
-            share     mine   = share_of(row, now.w != 0.0f);
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-            {
-                fetch(mine, j);
-                if (j % CHUNK == CHUNK - 1)
-                    commit();
-            }
-            if (now.id >= 0 && now.id < d.vocab)
-                now.s = to_float(static_cast<const T*>(d.logits)[row * d.logits_stride + now.id]);
-            if (several)
-                cluster_wait(); // every block of the cluster has started and made its barriers: its memory may be written
-            bool lost = false; // a wait for the other blocks has run out: rows are NaN from there on
-            for (int turn = 0; row < d.rows; row += step, ++turn, now = then)
-            {
-                const int    set  = turn & 1;
-                const T*     s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
-                T*           grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
-                const cut<T> c(s, d.vocab);
-                const int    loose = c.loose(tid, first, last && tid < 16);
-                float        one   = now.w != 0.0f && loose >= 0 ? to_float(s[loose]) : -inf;
-                const share  next  = share_of(row + step, w_then != 0.0f);
-                const float  w     = now.w;
-                then               = facts(row + step, w_then);
-                w_then             = weight(row + 2 * step);
-
-                // ---- the warps' part of the entries, and of the row's largest value and sum
-                int*  ids = ids_of[set];
-                float t = now.t, ew = 0.0f; // ew: of this entry, against the largest of its warp
-                if (warp * 32 < d.k)
-                {
-                    const float tm = warp_reduce(now.id >= 0 ? t : -inf, larger());
-                    t              = __fmul_rn(__fsub_rn(t, tm), L.c);
-                    ew             = now.id >= 0 ? pow2(t) : 0.0f;
-                    const float es  = warp_reduce(ew, add());
-                    const bool  odd = __any_sync(0xffffffffu, now.odd);
-                    if (tid < d.k)
-                        ids[tid] = now.id;
-                    if (lane == 0)
-                        part_t[warp] = make_float2(odd ? nan : tm, es);
-                }
-                if (MODE != GRAD)
-                {
-                    // from the lowest finite value on: a row of nothing but -infinity has the sum 0
-                    float  m = fmaxf(one, -3.40282347e38f);
-                    float2 z = make_float2(pow2(__fmul_rn(__fsub_rn(one, m), L.c)), 0.0f);
-#pragma unroll
-                    for (int q = 0; q < CHUNKS; ++q)
+                    const cut<T> c(s, d.vocab);
+                    const int    begin = min(rank * L.vectors, c.n), end = min(begin + L.vectors, c.n);
+                    const int    from = first ? 0 : c.head + begin * N, to = last ? d.vocab : c.head + end * N;
+                    float        top = -inf;
+                    bool         odd = false;
+#pragma unroll 4
+                    for (int k = lane; k < d.k; k += 32)
                     {
-                        if (MODE == LOSS)
-                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
-                        else if (q == 0)
-                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
-                        else if (q == 1)
-                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 2) : "memory");
-                        else if (q == 2)
-                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 3) : "memory");
-                        else
-                            asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        piece<T> x[CHUNK];
-                        if (q * CHUNK < mine.n)
-                        {
-                            float higher = m;
-#pragma unroll
-                            for (int i = 0; i < CHUNK; ++i)
-                            {
-                                if (q * CHUNK + i < mine.n)
-                                    vector(x[i], q * CHUNK + i);
-                                else
-                                    x[i].clear();
-                                higher = x[i].largest(higher);
-                            }
-                            const float scale = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
-                            z                 = mul2(z, make_float2(scale, scale));
-                            m                 = higher;
-#pragma unroll
-                            for (int i = 0; i < CHUNK; ++i)
-                                z = x[i].sum(z, m, L.c);
-                        }
-                        if (MODE == LOSS)
-                        {
-#pragma unroll
-                            for (int i = 0; i < CHUNK; ++i)
-                                fetch(next, q * CHUNK + i);
-                            commit();
-                        }
+                        int   id;
+                        float t;
+                        odd |= read_entry(d, r, k, id, t);
+                        e.id[k] = id;
+                        e.t[k]  = t;
+                        top     = fmaxf(top, t);
                     }
-                    const float wm = warp_reduce(m, larger());
-                    const float wz = warp_reduce(__fmul_rn(__fadd_rn(z.x, z.y), pow2(__fmul_rn(__fsub_rn(m, wm), L.c))), add());
-                    if (lane == 0)
-                        part[warp] = make_float2(wm, wz);
-                }
-                __syncthreads();
-                // the next row's logits at its ids
-                if (then.id >= 0 && then.id < d.vocab)
-                    then.s = to_float(s[step * d.logits_stride + then.id]);
-                if (warp == 0)
+#pragma unroll 4
+                    for (int k = lane; k < d.k; k += 32)
+                    {
+                        const int  id   = e.id[k];
+                        const bool here = id >= from && id < to;
+                        e.s[k]          = here || (MODE != GRAD && first && id >= 0 && id < d.vocab) ? to_float(s[id]) : 0.0f;
+                        if (!here && !(MODE != GRAD && first))
+                            e.s[k] = 0.0f;
+                    }
+                    top     = warp_reduce(top, larger());
+                    odd     = __any_sync(0xffffffffu, odd);
+                    a.found = odd || top != -inf;
+                    a.bad   = odd || !(top < inf);
+                    float sum = 0.0f;
+                    for (int k = lane; k < d.k; k += 32)
+                    {
+                        const float t = __fmul_rn(__fsub_rn(e.t[k], top), L.c);
+                        const float p = e.id[k] >= 0 ? pow2(t) : 0.0f;
+                        e.t[k]        = t;
+                        e.p[k]        = p;
+                        sum           = __fadd_rn(sum, p);
+                    }
+                    sum = warp_reduce(sum, add());
+                    for (int k = lane; k < d.k; k += 32)
+                        e.p[k] = __fdiv_rn(e.p[k], sum);
+                    a.esum2 = log2f(sum);
+                    return a;
+                };
+                float   w_then = weight(row + step);
+                facts   now    = prepare(row, weight(row), s, of_row[0]);
+                bool    lost   = false; // a wait for the other blocks has run out: rows are NaN from there on
+                for (int turn = 0; row < d.rows; row += step, ++turn)
                 {
-                    const float2 e    = lane * 32 < d.k ? part_t[lane & (EWARPS - 1)] : make_float2(-inf, 0.0f);
-                    const float  tmax = warp_reduce(e.x, larger());
-                    const bool   odd  = __any_sync(0xffffffffu, e.x != e.x);
-                    const float  esum = warp_reduce(e.x > -inf ? __fmul_rn(e.y, pow2(__fmul_rn(__fsub_rn(e.x, tmax), L.c))) : 0.0f, add());
-                    bool         bad  = odd || !(tmax < inf);
-                    float        top = 0.0f, z = 0.0f;
+                    const int      set = turn & 1;
+                    const entries& e   = of_row[set];
+                    const float    w_after = weight(row + 2 * step);
+                    float          top = 0.0f, z = 1.0f;
+                    bool           bad = now.bad;
                     if (MODE != GRAD)
                     {
-                        float2 o = lane * 32 < nt ? part[lane & 15] : make_float2(-3.40282347e38f, 0.0f);
-                        top      = warp_reduce(o.x, larger());
-                        z        = warp_reduce(__fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c))), add());
+                        bar_sync(SUMS, ALL);
+                        float2 o = lane < WARPS ? part[lane & (WARPS - 1)] : make_float2(lowest, 0.0f);
+                        if (MODE == LOSS)
+                        {
+                            __syncwarp();
+                            if (lane == 0)
+                                result.ahead = w_after != 0.0f;
+                            __syncwarp();
+                            bar_arrive(RESULT, ALL);
+                        }
+                        top = warp_reduce(o.x, larger());
+                        z   = warp_reduce(__fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c))), add());
                         if (several)
                         {
                             if (lane == 0)
@@ -724,111 +845,73 @@ namespace aeonb
                             __syncwarp();
                             if (lane < L.blocks)
                                 cluster_send(&theirs[set][rank], &arrived[set], lane, make_float2(top, z));
-                            lost |= lost || !barrier_wait(&arrived[set], (turn >> 1) & 1);
-                            bad |= lost;
-                            o   = lane < L.blocks ? theirs[set][lane & 15] : make_float2(-3.40282347e38f, 0.0f);
+                            lost = lost || !barrier_wait(&arrived[set], (turn >> 1) & 1);
+                            bad |= __any_sync(0xffffffffu, lost);
+                            o   = lane < L.blocks ? theirs[set][lane & 15] : make_float2(lowest, 0.0f);
                             top = warp_reduce(o.x, larger());
                             z   = warp_reduce(__fmul_rn(o.y, pow2(__fmul_rn(__fsub_rn(o.x, top), L.c))), add());
                         }
                         bad |= !(fabsf(top) < inf) || !(z > 0.0f);
                     }
-                    if (lane == 0)
+                    float f = 0.0f, fq = 0.0f, high = top;
+                    if (MODE != LOSS)
                     {
-                        result[0] = tmax;
-                        result[1] = esum;
-                        result[2] = top;
-                        result[3] = z;
-                        flags     = (odd || tmax != -inf ? 1 : 0) | (bad ? 2 : 0);
+                        f = __fmul_rn(__fmul_rn(now.w, L.factor), now.up);
+                        if (MODE == GRAD)
+                        {
+                            const float2 at = against_lse(L, now.lse);
+                            bad |= !(fabsf(now.lse) < inf);
+                            high = at.x;
+                            fq   = __fmul_rn(f, at.y);
+                        }
+                        else
+                            fq = __fdiv_rn(f, z);
+                        if (bad)
+                            fq = nan;
+                        if (lane == 0)
+                            result = outcome{high, fq, now.found, w_then != 0.0f};
+                        __syncwarp();
+                        bar_arrive(RESULT, ALL);
                     }
-                }
-                __syncthreads();
-                const bool  found = flags & 1;
-                bool        bad   = flags & 2;
-                const float tmax = result[0], esum = result[1];
-                float       top = result[2];
-                const float z   = result[3];
-                if (warp * 32 < d.k)
-                {
-                    const float shift = __fmul_rn(__fsub_rn(part_t[warp].x, tmax), L.c); // of the warp's largest entry
-                    const float p     = now.id >= 0 ? __fdiv_rn(__fmul_rn(ew, pow2(shift)), esum) : 0.0f;
-                    if (tid < d.k)
-                        probs[tid] = p;
                     if (MODE != GRAD && first)
                     {
-                        // p (log p - s / T + lse), to the base 2, but for the logarithms of the two sums
-                        float term = p > 0.0f ? __fmul_rn(p, __fadd_rn(__fadd_rn(t, shift), __fmul_rn(__fsub_rn(top, now.s), L.c))) : 0.0f;
-                        term       = warp_reduce(term, add());
-                        if (lane == 0)
-                            part_term[warp] = term;
-                    }
-                }
-                if (MODE != LOSS)
-                {
-                    T*    to = grad + c.head + (min(rank * L.vectors, c.n) + tid) * piece<T>::N;
-                    float f = 0.0f, fq = 0.0f;
-                    if (MODE == GRAD)
-                    {
-                        const float2 at = against_lse(L, now.lse);
-                        bad |= !(fabsf(now.lse) < inf);
-                        top = at.x;
-                        fq  = at.y;
-                    }
-                    if (found)
-                    {
-                        f  = bad ? nan : __fmul_rn(__fmul_rn(w, L.factor), now.up);
-                        fq = MODE == GRAD ? __fmul_rn(f, fq) : __fdiv_rn(f, z);
-                    }
-                    if (loose >= 0)
-                        grad[loose] = from_float<T>(found ? __fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one, top), L.c))) : 0.0f);
-                    const int written = share_of(row, true).n;
-#pragma unroll
-                    for (int q = 0; q < CHUNKS; ++q)
-                    {
-                        if (MODE == GRAD)
-                            asm volatile("cp.async.wait_group %0;" ::"n"(CHUNKS - 1) : "memory");
-#pragma unroll
-                        for (int i = 0; i < CHUNK; ++i)
+                        float loss = 0.0f, lse = 0.0f;
+                        if (now.found)
                         {
-                            const int j = q * CHUNK + i;
-                            if (j < written)
-                            {
-                                uint4 g = make_uint4(0, 0, 0, 0);
-                                if (found)
-                                {
-                                    piece<T> x;
-                                    vector(x, j);
-                                    g = x.gradient(top, L.c, fq);
-                                }
-                                store_piece(to + (int64_t)j * nt * piece<T>::N, g, L.together);
-                            }
-                            fetch(next, j);
+                            const float zsum2 = log2f(z);
+                            loss              = entries_loss(L, e, now.esum2, top, zsum2, now.w);
+                            loss              = bad ? nan : loss;
+                            lse               = bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2));
                         }
-                        commit();
+                        if (lane == 0)
+                            write_loss(d, row, loss, lse);
                     }
-                    __syncthreads();
-                    // ids of this block's values
-                    const int begin = min(rank * L.vectors, c.n), n = min(L.vectors, c.n - begin);
-                    const int from = first ? 0 : c.head + begin * piece<T>::N, end = last ? d.vocab : c.head + (begin + n) * piece<T>::N;
-                    if (found && !bad && now.id >= from && now.id < end)
-                        entry_gradient(L, ids, probs, grad, tid, now.id, now.s, top, f, fq);
-                }
-                else
-                    __syncthreads();
-                if (MODE != GRAD && first && tid == 0)
-                {
-                    float loss = 0.0f, lse = 0.0f;
-                    if (found)
+                    const facts here = now;
+                    now              = prepare(row + step, w_then, s + step * d.logits_stride, of_row[set ^ 1]);
+                    w_then           = w_after;
+                    if (MODE != LOSS)
                     {
-                        const float zsum2 = log2f(z);
-                        float       term  = __fsub_rn(zsum2, log2f(esum));
-                        for (int i = 0; i * 32 < d.k; ++i)
-                            term = __fadd_rn(term, part_term[i]);
-                        loss = bad ? nan : __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(term, LN2));
-                        lse  = bad ? nan : __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2));
+                        T*           grad = static_cast<T*>(d.grad) + row * d.grad_stride;
+                        const cut<T> c(s, d.vocab);
+                        const int    begin = min(rank * L.vectors, c.n), end = min(begin + L.vectors, c.n);
+                        const int    from = first ? 0 : c.head + begin * N, to = last ? d.vocab : c.head + end * N;
+                        const bool   twice = here.found && !bad && repeats(e.id, table, d.k);
+                        bar_sync(WRITTEN, ALL);
+                        if (here.found && !bad)
+                            for (int k = lane; k < d.k; k += 32)
+                            {
+                                const int id = e.id[k];
+                                if (id < from || id >= to)
+                                    continue;
+                                if (twice)
+                                    entry_gradient(L, e.id, e.p, grad, k, id, e.s[k], high, f, fq);
+                                else
+                                    grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(e.s[k], high), L.c))), __fmul_rn(f, e.p[k])));
+                            }
+                        __syncwarp();
                     }
-                    write_loss(d, row, loss, lse);
+                    s += step * d.logits_stride;
                 }
-                mine = next;
             }
             if (several) // nothing is sent to a block that has left
             {
@@ -957,16 +1040,14 @@ namespace aeonb
             return cudaGetLastError();
         }
 
-        template <typename T, int MODE>
+        template <typename T, int MODE, int NT>
         cudaError_t launch_blocks(const distill_launch& L, cudaStream_t stream)
         {
-            auto                kernel = distill_block_kernel<T, MODE>;
+            auto                kernel = distill_block_kernel<T, MODE, NT>;
             cudaLaunchConfig_t  cfg    = {};
             cudaLaunchAttribute attr   = {};
-            // a thread for each NV vectors of a block, and for each entry
-            const int warps      = std::min(16, std::max(ENTRIES / 32, (L.vectors + BLOCK_VECTORS * 32 - 1) / (BLOCK_VECTORS * 32)));
-            cfg.blockDim         = dim3(warps * 32);
-            cfg.dynamicSmemBytes = BLOCK_VECTORS * warps * 32 * 16;
+            cfg.blockDim         = dim3(NT + 32);
+            cfg.dynamicSmemBytes = BLOCK_VECTORS * NT * 16;
             cfg.stream           = stream;
             const bool cluster   = MODE != GRAD && L.blocks > 1;
             if (cluster)
@@ -978,7 +1059,7 @@ namespace aeonb
                 cfg.numAttrs = 1;
             }
             // rows at once: the groups of a row's blocks that find room together, asked for once per kernel, size and device
-            static std::atomic<int> room[64][17][5];
+            static std::atomic<int> room[64][5];
             int                     size = 0; // log2 of the cluster's blocks
             while (cluster && 1 << size < L.blocks)
                 ++size;
@@ -987,10 +1068,10 @@ namespace aeonb
             if (e != cudaSuccess)
                 return e;
             if (device < 64)
-                groups = room[device][warps][size].load(std::memory_order_acquire);
+                groups = room[device][size].load(std::memory_order_acquire);
             if (groups == 0)
             {
-                if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BLOCK_VECTORS * 512 * 16)) != cudaSuccess ||
+                if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes)) != cudaSuccess ||
                     (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
                     return e;
                 cfg.gridDim = dim3(cluster ? L.blocks : 1);
@@ -999,7 +1080,7 @@ namespace aeonb
                 else
                 {
                     int sms = 0;
-                    e       = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&groups, kernel, warps * 32, cfg.dynamicSmemBytes);
+                    e       = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&groups, kernel, NT + 32, cfg.dynamicSmemBytes);
                     if (e == cudaSuccess)
                         e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
                     groups *= sms;
@@ -1009,7 +1090,7 @@ namespace aeonb
                 if (groups < 1)
                     return cudaErrorInvalidConfiguration;
                 if (device < 64)
-                    room[device][warps][size].store(groups, std::memory_order_release);
+                    room[device][size].store(groups, std::memory_order_release);
             }
             if (!cluster)
                 groups = std::max(1, groups / L.blocks);
@@ -1049,7 +1130,7 @@ namespace aeonb
             }
             L.blocks  = (int)blocks;
             L.vectors = (int)(((vectors + blocks - 1) / blocks + 7) / 8 * 8); // whole lines of 128 bytes
-            return launch_blocks<T, MODE>(L, stream);
+            return L.vectors <= BLOCK_VECTORS * 256 ? launch_blocks<T, MODE, 256>(L, stream) : launch_blocks<T, MODE, 512>(L, stream);
         }
 
         template <typename T>
