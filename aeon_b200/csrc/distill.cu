@@ -1116,9 +1116,13 @@ namespace aeonb
                 return launch_warps<T, MODE, 256, 4, true>(L, stream);
             if (vectors <= 32 * 8)
                 return launch_warps<T, MODE, 256, 8, true>(L, stream);
-            // blocks of a row: as many as hold it, and more while they do not fill the SMs and have 4 KB each
-            constexpr int most   = BLOCK_VECTORS * 512;
-            int64_t       blocks = 1;
+            // Threads of a block: 256 where there is a gradient and up to eight such blocks hold a row, else 512.  8192 rows of 131072 bf16
+            // logits, 256 / 512: with gradient 0.88 / 0.91 ms, gradient alone 0.74 / 0.80, loss alone 0.51 / 0.47 (where nothing waits for
+            // the other blocks, fewer of them cost less).
+            const bool    narrow = MODE == GRAD || (MODE == LOSS_GRAD && vectors <= 8 * BLOCK_VECTORS * 256);
+            const int64_t most   = BLOCK_VECTORS * (narrow ? 256 : 512);
+            // Blocks of a row: as many as hold it, and more while they do not fill the SMs and have 4 KB each.
+            int64_t blocks = 1;
             while (blocks * most < vectors)
                 blocks *= 2;
             while (blocks < 8 && L.d.rows * blocks < 148 && vectors / (blocks * 2) >= 256)
@@ -1130,7 +1134,10 @@ namespace aeonb
             }
             L.blocks  = (int)blocks;
             L.vectors = (int)(((vectors + blocks - 1) / blocks + 7) / 8 * 8); // whole lines of 128 bytes
-            return L.vectors <= BLOCK_VECTORS * 256 ? launch_blocks<T, MODE, 256>(L, stream) : launch_blocks<T, MODE, 512>(L, stream);
+            if constexpr (MODE != GRAD)
+                if (L.vectors > BLOCK_VECTORS * 256)
+                    return launch_blocks<T, MODE, 512>(L, stream);
+            return launch_blocks<T, MODE, 256>(L, stream);
         }
 
         template <typename T>

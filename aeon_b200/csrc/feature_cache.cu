@@ -1,13 +1,16 @@
 // The feature cache on sm_100a: rows of floats to 8-bit codes in pages, with a scale for each token and head, and back.
 //
-// A warp per group (token and head): it looks up the page, takes the largest magnitude of the group's values, and writes the
-// codes.  The quotient x / scale is first formed as x times the reciprocal; where that lies so near to the middle between
-// two codes that the roundings of the two operations could decide, the exact quotient does (in 64 bits: the numerator and
-// denominator have 24 bits each, so a quotient that is not in the middle is at least 2^-25 of it away, and the division's
-// own rounding cannot carry it there).
+// A group (token and head) is read once: up to 32 lanes hold a chunk each, of 32 bytes of the rows where their place allows it, else 16,
+// else one value; several groups share a warp.  Its largest magnitude is that of the bit patterns without their sign; only where
+// that is no finite number are infinities looked at one by one.  Floor: the bytes of rows, codes and scales.
+//
+// The quotient x / scale is formed as x times the reciprocal, off by 2^-23 of itself at most; where it lies so near to the
+// middle between two codes that this could decide, the exact quotient does (in 64 bits: numerator and denominator have 24 bits
+// each, so a quotient that is not in the middle is at least 2^-25 of it away, and the division's own rounding cannot carry it there).
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "float_rows.cuh"
 
@@ -17,28 +20,29 @@ namespace aeonb
     {
         constexpr uint32_t ABS_BITS = 0x7fffffffu, INF_BITS = 0x7f800000u, MINUS_INF = 0xff800000u;
 
+        struct cache_launch
+        {
+            aeonb_cache_desc d;
+            int              lanes;  // of a group
+            int              groups; // of a sequence
+        };
+
         // Where a group's codes and scale lie; -1 for a token without a place.
         __device__ __forceinline__ int64_t group_place(const aeonb_cache_desc& d, int seq, int token, int head)
         {
             const int64_t at = (int64_t)token + (d.start ? d.start[seq] : 0);
             if (at < 0 || at >= (int64_t)d.table_pages * d.page_tokens)
                 return -1;
-            const int32_t page = d.table[seq * d.table_stride + at / d.page_tokens];
+            const uint32_t page_of = (uint32_t)at / (uint32_t)d.page_tokens; // a position is below 2^32
+            const int32_t  page    = d.table[seq * d.table_stride + page_of];
             if (page < 0 || page >= d.pages)
                 return -1;
-            return ((int64_t)page * d.page_tokens + at % d.page_tokens) * d.heads + head;
+            return ((int64_t)page * d.page_tokens + ((uint32_t)at - page_of * (uint32_t)d.page_tokens)) * d.heads + head;
         }
 
         __device__ __forceinline__ int tokens_of(const aeonb_cache_desc& d, int seq)
         {
             return d.length ? min(max(d.length[seq], 0), d.tokens) : d.tokens;
-        }
-
-        // bits of |x| that count in the group's largest magnitude: none of -infinity, NaN and +infinity as they are
-        __device__ __forceinline__ uint32_t magnitude(float x)
-        {
-            const uint32_t b = __float_as_uint(x);
-            return b == MINUS_INF ? 0u : b & ABS_BITS;
         }
 
         template <int CODE>
@@ -53,34 +57,26 @@ namespace aeonb
             return s;
         }
 
+        // The code of one value, whatever it is.
         template <int CODE>
-        __device__ __forceinline__ uint8_t encode(float x, float scale, float inverse)
+        __device__ __noinline__ uint32_t encode_exactly(float x, float scale)
         {
+            if (!(scale == scale))
+                return 0;
             if (__float_as_uint(x) == MINUS_INF)
                 return CODE == AEONB_CODE_INT8 ? 0x80 : 0xff;
-            const float t = __fmul_rn(x, inverse); // off by 2^-23 of itself at most
+            const double q = __ddiv_rn((double)x, (double)scale);
             if (CODE == AEONB_CODE_INT8)
-            {
-                float q = rintf(t);
-                if (fabsf(__fsub_rn(t, q)) > 0.5f - 0x1p-15f)
-                    q = (float)rint(__ddiv_rn((double)x, (double)scale));
-                return (uint8_t)(int8_t)(int)q;
-            }
-            const uint32_t low  = __float_as_uint(t) & 0xfffffu; // the bits behind the three that a normal e4m3 keeps
-            float          odd  = t;
-            if (low - 0x7fff8u <= 16u || (fabsf(t) < 0x1p-6f && t != 0.0f))
-            {
-                // the exact quotient, cut to float with its last bit set where bits were lost: rounds to e4m3 as it would itself
-                const double q = __ddiv_rn((double)x, (double)scale);
-                odd            = __double2float_rz(q);
-                if ((double)odd != q)
-                    odd = __uint_as_float(__float_as_uint(odd) | 1u);
-            }
-            return (uint8_t)__nv_cvt_float_to_fp8(odd, __NV_SATFINITE, __NV_E4M3);
+                return (uint32_t)(int)rint(q) & 0xff;
+            // cut to float with the last bit set where bits were lost: rounds to e4m3 as the quotient itself would
+            float odd = __double2float_rz(q);
+            if ((double)odd != q)
+                odd = __uint_as_float(__float_as_uint(odd) | 1u);
+            return __nv_cvt_float_to_fp8(odd, __NV_SATFINITE, __NV_E4M3);
         }
 
         template <int CODE>
-        __device__ __forceinline__ float decode(uint8_t code, float scale)
+        __device__ __forceinline__ float decode(uint32_t code, float scale)
         {
             if (CODE == AEONB_CODE_INT8)
                 return code == 0x80 ? __uint_as_float(MINUS_INF) : __fmul_rn((float)(int8_t)code, scale);
@@ -89,72 +85,419 @@ namespace aeonb
             return __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3))), scale);
         }
 
-        template <typename T, int CODE>
-        __global__ void __launch_bounds__(256) cache_write_kernel(const aeonb_cache_desc d)
+        __device__ __forceinline__ float2 mul2(float2 a, float b)
         {
-            const int64_t groups = (int64_t)d.seqs * d.tokens * d.heads;
-            const int     lane   = threadIdx.x & 31;
-            for (int64_t g = blockIdx.x * (int64_t)(blockDim.x / 32) + threadIdx.x / 32; g < groups; g += (int64_t)gridDim.x * (blockDim.x / 32))
+            float2 r;
+            asm("{ .reg .b64 t, u;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %4};\n"
+                "mul.rn.f32x2 t, t, u;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b));
+            return r;
+        }
+        __device__ __forceinline__ float2 add2(float2 a, float2 b)
+        {
+            float2 r;
+            asm("{ .reg .b64 t, u;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %5};\n"
+                "add.rn.f32x2 t, t, u;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+            return r;
+        }
+
+        // Codes of four values at once (in the order of the bytes); `exact` is set where one lies too near to a middle to tell.
+        template <int CODE>
+        __device__ __forceinline__ uint32_t encode4(float2 a, float2 b, float inverse, bool& exact)
+        {
+            const float2 s = mul2(a, inverse), t = mul2(b, inverse);
+            if (CODE == AEONB_CODE_INT8)
             {
-                const int head = (int)(g % d.heads), token = (int)(g / d.heads % d.tokens), seq = (int)(g / d.heads / d.tokens);
-                if (token >= tokens_of(d, seq))
-                    continue;
-                const int64_t place = group_place(d, seq, token, head);
-                if (place < 0)
+                const float  magic = 12582912.0f; // 1.5 2^23: the sum's last bits are the nearest integer
+                const float2 up = make_float2(magic, magic), down = make_float2(-magic, -magic);
+                const float2 p = add2(s, up), q = add2(t, up);
+                const float2 r = add2(p, down), u = add2(q, down);
+                const float2 e = add2(s, make_float2(-r.x, -r.y)), f = add2(t, make_float2(-u.x, -u.y));
+                exact |= fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y))) > 0.5f - 0x1p-15f;
+                const uint32_t lo = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040),
+                               hi = __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040);
+                return __byte_perm(lo, hi, 0x5410);
+            }
+            const float v[4] = {s.x, s.y, t.x, t.y};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) // the bits behind the three that a normal e4m3 keeps; below 2^-6 it keeps fewer
+                exact |= (__float_as_uint(v[i]) & 0xfffffu) - 0x7fff8u <= 16u || (fabsf(v[i]) < 0x1p-6f && v[i] != 0.0f);
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
+            return lo | hi << 16;
+        }
+
+        // Whether one of four codes stands for no finite number.
+        template <int CODE>
+        __device__ __forceinline__ bool odd4(uint32_t w)
+        {
+            if (CODE == AEONB_CODE_INT8)
+            {
+                const uint32_t v = w ^ 0x80808080u; // a byte of 0?
+                return ((v - 0x01010101u) & ~v & 0x80808080u) != 0;
+            }
+            return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+        }
+
+        // The numbers (not yet scaled) of four codes, all of them finite.
+        template <int CODE>
+        __device__ __forceinline__ void numbers4(uint32_t w, float2& a, float2& b)
+        {
+            if (CODE == AEONB_CODE_INT8)
+            {
+                w ^= 0x80808080u; // code + 128, as the last byte of 2^23 + code + 128
+                const float2 bias = make_float2(-8388736.0f, -8388736.0f);
+                a = add2(make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7541))), bias);
+                b = add2(make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7542)), __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7543))), bias);
+                return;
+            }
+            a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
+            b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+        }
+
+        // V values of a row in one lane's registers, and how they get there and away.
+        template <typename T, int V>
+        struct chunk
+        {
+            static constexpr int  W    = V * sizeof(T) / 4; // words
+            static constexpr bool WIDE = sizeof(T) == 4;
+            uint32_t              w[W];
+            __device__ __forceinline__ void load(const T* p)
+            {
+                if constexpr (W == 8)
+                    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                                 : "l"(p)
+                                 : "memory");
+                else
                 {
-                    if (lane == 0 && d.status)
-                        *d.status = 1;
-                    continue;
+                    const uint4 q = *reinterpret_cast<const uint4*>(p);
+                    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
                 }
-                const T* x = static_cast<const T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
-                T*       v = d.values ? static_cast<T*>(d.values) + seq * d.value_stride_seq + token * d.value_stride_token + head * d.value_stride_head
-                                      : nullptr;
-                uint32_t largest = 0;
-                for (int i = lane; i < d.dim; i += 32)
-                    largest = max(largest, magnitude(to_float(x[i])));
-                largest           = __reduce_max_sync(0xffffffffu, largest);
-                const float scale = group_scale<CODE>(largest), inverse = __frcp_rn(scale);
-                uint8_t*    codes = static_cast<uint8_t*>(d.codes) + place * d.dim;
-                if (lane == 0)
-                    d.scales[place] = scale;
-                for (int i = lane; i < d.dim; i += 32)
+            }
+            __device__ __forceinline__ void store(T* p) const
+            {
+                if constexpr (W == 8)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                 : "memory");
+                else
+                    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __device__ __forceinline__ void fill(float v)
+            {
+                const T one = from_float<T>(v);
+                uint32_t bits;
+                if constexpr (WIDE)
+                    bits = *reinterpret_cast<const uint32_t*>(&one);
+                else
+                    bits = *reinterpret_cast<const uint16_t*>(&one) * 0x10001u;
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    w[i] = bits;
+            }
+            __device__ __forceinline__ float2 pair(int i) const
+            {
+                if constexpr (WIDE)
+                    return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+                else if constexpr (std::is_same<T, __half>::value)
+                    return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                else
+                    return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            }
+            __device__ __forceinline__ void set(int i, float2 v)
+            {
+                if constexpr (WIDE)
+                    w[2 * i] = __float_as_uint(v.x), w[2 * i + 1] = __float_as_uint(v.y);
+                else if constexpr (std::is_same<T, __half>::value)
                 {
-                    const uint8_t q = scale == scale ? encode<CODE>(to_float(x[i]), scale, inverse) : (uint8_t)0;
-                    codes[i]        = q;
-                    if (v)
-                        v[i] = from_float<T>(decode<CODE>(q, scale));
+                    const __half2 h = __floats2half2_rn(v.x, v.y);
+                    w[i]            = *reinterpret_cast<const uint32_t*>(&h);
                 }
+                else
+                {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+                    w[i]                   = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            // bits of the largest magnitude as a float's, infinities and NaN among them
+            __device__ __forceinline__ uint32_t largest() const
+            {
+                if constexpr (WIDE)
+                {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        m = max(m, w[i] & ABS_BITS);
+                    return m;
+                }
+                else
+                {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+                    m = max(m & 0xffffu, m >> 16);
+                    if constexpr (std::is_same<T, __half>::value)
+                        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+                    else
+                        return m << 16;
+                }
+            }
+            __device__ __forceinline__ float value(int i) const
+            {
+                const float2 v = pair(i / 2);
+                return i & 1 ? v.y : v.x;
+            }
+        };
+
+        // One value: rows that lie on no 16 bytes.
+        template <typename T>
+        struct chunk<T, 1>
+        {
+            float v;
+            __device__ __forceinline__ void     load(const T* p) { v = to_float(*p); }
+            __device__ __forceinline__ void     store(T* p) const { *p = from_float<T>(v); }
+            __device__ __forceinline__ void     fill(float x) { v = x; }
+            __device__ __forceinline__ uint32_t largest() const { return __float_as_uint(v) & ABS_BITS; }
+            __device__ __forceinline__ float    value(int) const { return v; }
+        };
+
+        // The largest magnitude among a group's lanes, L of them from lane `base` on (any L: the largest of some values does not
+        // mind which of them it has seen twice).
+        __device__ __forceinline__ uint32_t group_largest(uint32_t m, int L, int base, int l)
+        {
+            if (L == 32)
+                return __reduce_max_sync(0xffffffffu, m);
+            for (int o = 1; o < L; o *= 2)
+            {
+                int from = l + o;
+                from     = from >= L ? from - L : from;
+                m        = max(m, __shfl_sync(0xffffffffu, m, base + from));
+            }
+            return m;
+        }
+
+        template <typename T, int CODE, int V>
+        __device__ __forceinline__ void decode_words(chunk<T, V>& x, const uint32_t* q, float scale)
+        {
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i)
+            {
+                float2 a, b;
+                odd |= odd4<CODE>(q[i]);
+                numbers4<CODE>(q[i], a, b);
+                x.set(2 * i, mul2(a, scale));
+                x.set(2 * i + 1, mul2(b, scale));
+            }
+            if (odd)
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i)
+                {
+                    x.set(2 * i, make_float2(decode<CODE>(q[i] & 0xff, scale), decode<CODE>(q[i] >> 8 & 0xff, scale)));
+                    x.set(2 * i + 1, make_float2(decode<CODE>(q[i] >> 16 & 0xff, scale), decode<CODE>(q[i] >> 24, scale)));
+                }
+        }
+
+        // Codes of a chunk, written; the chunk then holds the values that they stand for.
+        template <typename T, int CODE, int V>
+        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, float scale, float inverse, bool finite, uint8_t* codes)
+        {
+            if constexpr (V == 1)
+            {
+                bool     exact = !finite;
+                uint32_t q     = encode4<CODE>(make_float2(x.v, 0.0f), make_float2(0.0f, 0.0f), inverse, exact) & 0xff;
+                if (exact)
+                    q = encode_exactly<CODE>(x.v, scale);
+                *codes = (uint8_t)q;
+                x.v              = decode<CODE>(q, scale);
+            }
+            else
+            {
+                uint32_t q[V / 4];
+                bool     exact = !finite;
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i)
+                    q[i] = encode4<CODE>(x.pair(2 * i), x.pair(2 * i + 1), inverse, exact);
+                if (exact)
+#pragma unroll
+                    for (int i = 0; i < V / 4; ++i)
+                    {
+                        const float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
+                        q[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
+                               encode_exactly<CODE>(b.y, scale) << 24;
+                    }
+                if constexpr (V == 16)
+                    *reinterpret_cast<uint4*>(codes) = make_uint4(q[0], q[1], q[2], q[3]);
+                else if constexpr (V == 8)
+                    *reinterpret_cast<uint2*>(codes) = make_uint2(q[0], q[1]);
+                else
+                    *reinterpret_cast<uint32_t*>(codes) = q[0];
+                decode_words<T, CODE, V>(x, q, scale);
             }
         }
 
-        template <typename T, int CODE>
-        __global__ void __launch_bounds__(256) cache_read_kernel(const aeonb_cache_desc d)
+        // NC chunks a lane; 0: as many as it takes, read a second time for their codes.
+        template <typename T, int CODE, int V, int NC>
+        __global__ void __launch_bounds__(256) cache_write_kernel(const cache_launch L)
         {
-            const int64_t groups = (int64_t)d.seqs * d.tokens * d.heads;
-            const int     lane   = threadIdx.x & 31;
-            for (int64_t g = blockIdx.x * (int64_t)(blockDim.x / 32) + threadIdx.x / 32; g < groups; g += (int64_t)gridDim.x * (blockDim.x / 32))
+            const aeonb_cache_desc& d      = L.d;
+            const int               lane   = threadIdx.x & 31, mine = lane / L.lanes, base = mine * L.lanes, l = lane - base, at_once = 32 / L.lanes;
+            const int               group  = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * at_once + mine;
+            const int               token  = (uint32_t)group / (uint32_t)d.heads, head = group - token * d.heads;
+            const int               chunks = d.dim / V;
+            for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
-                const int head = (int)(g % d.heads), token = (int)(g / d.heads % d.tokens), seq = (int)(g / d.heads / d.tokens);
-                T*        v = static_cast<T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
-                if (token >= tokens_of(d, seq))
+                const bool    there = mine < at_once && group < L.groups && token < tokens_of(d, seq);
+                const int64_t place = there ? group_place(d, seq, token, head) : -1;
+                if (there && place < 0 && l == 0 && d.status)
+                    *d.status = 1;
+                const T*    x = static_cast<const T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
+                chunk<T, V> c[NC ? NC : 1];
+                uint32_t    m = 0;
+                if (place >= 0)
                 {
-                    for (int i = lane; i < d.dim; i += 32)
-                        v[i] = from_float<T>(0.0f);
-                    continue;
+                    if constexpr (NC > 0)
+                    {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            if (j * L.lanes + l < chunks)
+                            {
+                                c[j].load(x + (j * L.lanes + l) * V);
+                                m = max(m, c[j].largest());
+                            }
+                    }
+                    else
+                        for (int i = l; i < chunks; i += L.lanes)
+                        {
+                            c[0].load(x + (int64_t)i * V);
+                            m = max(m, c[0].largest());
+                        }
                 }
-                const int64_t place = group_place(d, seq, token, head);
+                m                 = group_largest(m, L.lanes, base, l);
+                const bool finite = m < INF_BITS;
+                if (__any_sync(0xffffffffu, !finite))
+                {
+                    // an infinity or NaN somewhere in the warp: the largest without -infinity
+                    uint32_t   n   = 0;
+                    const auto see = [&](float v) {
+                        if (__float_as_uint(v) != MINUS_INF)
+                            n = max(n, __float_as_uint(v) & ABS_BITS);
+                    };
+                    if (place >= 0)
+                    {
+                        if constexpr (NC > 0)
+                        {
+#pragma unroll
+                            for (int j = 0; j < NC; ++j)
+                                if (j * L.lanes + l < chunks)
+#pragma unroll
+                                    for (int i = 0; i < V; ++i)
+                                        see(c[j].value(i));
+                        }
+                        else
+                            for (int64_t i = l; i < d.dim; i += L.lanes)
+                                see(to_float(x[i]));
+                    }
+                    m = group_largest(n, L.lanes, base, l);
+                }
+                if (place < 0)
+                    continue;
+                const float scale = group_scale<CODE>(m), inverse = __frcp_rn(scale);
+                if (l == 0)
+                    d.scales[place] = scale;
+                uint8_t* codes = static_cast<uint8_t*>(d.codes) + place * d.dim;
+                T*       v     = d.values ? static_cast<T*>(d.values) + seq * d.value_stride_seq + token * d.value_stride_token + head * d.value_stride_head
+                                          : nullptr;
+                if constexpr (NC > 0)
+                {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+                        if (j * L.lanes + l < chunks)
+                        {
+                            const int at = (j * L.lanes + l) * V;
+                            encode_chunk<T, CODE, V>(c[j], scale, inverse, finite, codes + at);
+                            if (v)
+                                c[j].store(v + at);
+                        }
+                }
+                else
+                    for (int i = l; i < chunks; i += L.lanes)
+                    {
+                        const int64_t at = (int64_t)i * V;
+                        c[0].load(x + at);
+                        encode_chunk<T, CODE, V>(c[0], scale, inverse, finite, codes + at);
+                        if (v)
+                            c[0].store(v + at);
+                    }
+            }
+        }
+
+        template <typename T, int CODE, int V>
+        __global__ void __launch_bounds__(256) cache_read_kernel(const cache_launch L)
+        {
+            const aeonb_cache_desc& d     = L.d;
+            const int               lane  = threadIdx.x & 31, mine = lane / L.lanes, l = lane - mine * L.lanes, at_once = 32 / L.lanes;
+            const int               group = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * at_once + mine;
+            const int               token = (uint32_t)group / (uint32_t)d.heads, head = group - token * d.heads;
+            const int               chunks = d.dim / V;
+            if (mine >= at_once || group >= L.groups)
+                return;
+            for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
+            {
+                T*          v = static_cast<T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
+                chunk<T, V> c;
+                int64_t     place = -1;
+                if (token < tokens_of(d, seq))
+                {
+                    place = group_place(d, seq, token, head);
+                    c.fill(__uint_as_float(0x7fffffffu));
+                    if (place < 0 && l == 0 && d.status)
+                        *d.status = 1;
+                }
+                else
+                    c.fill(0.0f);
                 if (place < 0)
                 {
-                    if (lane == 0 && d.status)
-                        *d.status = 1;
-                    for (int i = lane; i < d.dim; i += 32)
-                        v[i] = from_float<T>(__uint_as_float(0x7fffffffu));
+                    for (int i = l; i < chunks; i += L.lanes)
+                        c.store(v + (int64_t)i * V);
                     continue;
                 }
                 const float    scale = d.scales[place];
                 const uint8_t* codes = static_cast<const uint8_t*>(d.codes) + place * d.dim;
-                for (int i = lane; i < d.dim; i += 32)
-                    v[i] = from_float<T>(decode<CODE>(codes[i], scale));
+                for (int i = l; i < chunks; i += L.lanes)
+                {
+                    const uint8_t* q = codes + (int64_t)i * V;
+                    if constexpr (V == 1)
+                        c.v = decode<CODE>(*q, scale);
+                    else
+                    {
+                        uint32_t w[V / 4];
+                        if constexpr (V == 16)
+                        {
+                            const uint4 u = __ldcs(reinterpret_cast<const uint4*>(q));
+                            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                        }
+                        else if constexpr (V == 8)
+                        {
+                            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(q));
+                            w[0] = u.x, w[1] = u.y;
+                        }
+                        else
+                            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
+                        decode_words<T, CODE, V>(c, w, scale);
+                    }
+                    c.store(v + (int64_t)i * V);
+                }
             }
         }
 
@@ -208,15 +551,67 @@ namespace aeonb
                 throw std::invalid_argument("negative stride");
         }
 
-        template <typename T>
-        void launch_cache(const aeonb_cache_desc& d, bool write, unsigned blocks, cudaStream_t stream)
+        template <typename T, int CODE, int V>
+        void launch_chunks(cache_launch& L, bool write, cudaStream_t stream)
         {
-            if (write)
-                d.code == AEONB_CODE_INT8 ? cache_write_kernel<T, AEONB_CODE_INT8><<<blocks, 256, 0, stream>>>(d)
-                                          : cache_write_kernel<T, AEONB_CODE_E4M3><<<blocks, 256, 0, stream>>>(d);
+            const int chunks = L.d.dim / V;
+            L.lanes          = std::min(chunks, 32);
+            const int warps  = (int)std::min<int64_t>(8, ((int64_t)L.groups + 32 / L.lanes - 1) / (32 / L.lanes));
+            const int each   = warps * (32 / L.lanes);
+            const dim3 grid((unsigned)(((int64_t)L.groups + each - 1) / each), (unsigned)std::min(L.d.seqs, 65535));
+            if (!write)
+                cache_read_kernel<T, CODE, V><<<grid, warps * 32, 0, stream>>>(L);
+            else if (chunks <= 32)
+                cache_write_kernel<T, CODE, V, 1><<<grid, warps * 32, 0, stream>>>(L);
+            else if (chunks <= 32 * 4)
+                cache_write_kernel<T, CODE, V, 4><<<grid, warps * 32, 0, stream>>>(L);
             else
-                d.code == AEONB_CODE_INT8 ? cache_read_kernel<T, AEONB_CODE_INT8><<<blocks, 256, 0, stream>>>(d)
-                                          : cache_read_kernel<T, AEONB_CODE_E4M3><<<blocks, 256, 0, stream>>>(d);
+                cache_write_kernel<T, CODE, V, 0><<<grid, warps * 32, 0, stream>>>(L);
+        }
+
+        // bytes that every group's first value lies on
+        template <typename T>
+        int rows_lie_on(const aeonb_cache_desc& d, bool write)
+        {
+            uintptr_t all = (uintptr_t)d.rows | (uintptr_t)d.dim * sizeof(T);
+            if (d.seqs > 1)
+                all |= (uintptr_t)d.row_stride_seq * sizeof(T);
+            if (d.tokens > 1)
+                all |= (uintptr_t)d.row_stride_token * sizeof(T);
+            if (d.heads > 1)
+                all |= (uintptr_t)d.row_stride_head * sizeof(T);
+            if (write && d.values)
+            {
+                all |= (uintptr_t)d.values;
+                if (d.seqs > 1)
+                    all |= (uintptr_t)d.value_stride_seq * sizeof(T);
+                if (d.tokens > 1)
+                    all |= (uintptr_t)d.value_stride_token * sizeof(T);
+                if (d.heads > 1)
+                    all |= (uintptr_t)d.value_stride_head * sizeof(T);
+            }
+            // the codes of a chunk lie on as many bytes as it has values
+            const uintptr_t codes = ((uintptr_t)d.codes | (uintptr_t)d.dim);
+            if (all % 32 == 0 && codes % (32 / sizeof(T)) == 0)
+                return 32;
+            return all % 16 == 0 && codes % (16 / sizeof(T)) == 0 ? 16 : 1;
+        }
+
+        template <typename T, int CODE>
+        void launch_code(cache_launch& L, bool write, cudaStream_t stream)
+        {
+            switch (rows_lie_on<T>(L.d, write))
+            {
+            case 32: launch_chunks<T, CODE, 32 / sizeof(T)>(L, write, stream); break;
+            case 16: launch_chunks<T, CODE, 16 / sizeof(T)>(L, write, stream); break;
+            default: launch_chunks<T, CODE, 1>(L, write, stream); break;
+            }
+        }
+
+        template <typename T>
+        void launch_cache(cache_launch& L, bool write, cudaStream_t stream)
+        {
+            L.d.code == AEONB_CODE_INT8 ? launch_code<T, AEONB_CODE_INT8>(L, write, stream) : launch_code<T, AEONB_CODE_E4M3>(L, write, stream);
         }
 
         int run_cache(aeonb_ctx* ctx, const aeonb_cache_desc* desc, bool write)
@@ -228,17 +623,19 @@ namespace aeonb
                 check_cache(d, write);
                 if (d.seqs == 0 || d.tokens == 0)
                     return AEONB_OK;
+                if ((int64_t)d.tokens * d.heads > 0x7fffff00)
+                    throw error(AEONB_ERR_UNSUPPORTED, "more tokens and heads of a sequence than a launch takes");
                 device_scope   scope(ctx->device);
+                cache_launch   L{d, 0, d.tokens * d.heads};
                 const int64_t  groups = (int64_t)d.seqs * d.tokens * d.heads;
-                const unsigned blocks = (unsigned)std::min<int64_t>((groups + 7) / 8, 148 * 64);
                 const int64_t  values = groups * d.dim;
                 const cudaStream_t stream = d.stream ? static_cast<cudaStream_t>(d.stream) : ctx->stream;
                 launch_timer   timer(ctx, AEONB_KERNEL_OTHER, values * (float_size(d.dtype) * (d.values && write ? 2 : 1) + 1) + groups * 4, stream);
                 switch (d.dtype)
                 {
-                case AEONB_F32: launch_cache<float>(d, write, blocks, stream); break;
-                case AEONB_F16: launch_cache<__half>(d, write, blocks, stream); break;
-                case AEONB_BF16: launch_cache<__nv_bfloat16>(d, write, blocks, stream); break;
+                case AEONB_F32: launch_cache<float>(L, write, stream); break;
+                case AEONB_F16: launch_cache<__half>(L, write, stream); break;
+                case AEONB_BF16: launch_cache<__nv_bfloat16>(L, write, stream); break;
                 }
                 const cudaError_t e = cudaGetLastError();
                 if (e != cudaSuccess)
