@@ -4,9 +4,10 @@
 // else one value; several groups share a warp.  Its largest magnitude is that of the bit patterns without their sign; only where
 // that is no finite number are infinities looked at one by one.  Floor: the bytes of rows, codes and scales.
 //
-// The quotient x / scale is formed as x times the reciprocal, off by 2^-23 of itself at most; where it lies so near to the
-// middle between two codes that this could decide, the exact quotient does (in 64 bits: numerator and denominator have 24 bits
-// each, so a quotient that is not in the middle is at least 2^-25 of it away, and the division's own rounding cannot carry it there).
+// Codes are those of the exact quotient x / scale.  It is formed as x times the reciprocal and corrected by its own remainder once, which
+// gives the quotient of 24 bits; one in the middle between two codes then is exactly there and goes to the even code.  What remains
+// is a quotient that is only rounded to the middle (often so in 16-bit rows, whose values and largest value are ratios of small
+// numbers, but for the rounding of the scale): the sign of the remainder behind it tells on which side it lies.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -20,20 +21,36 @@ namespace aeonb
     {
         constexpr uint32_t ABS_BITS = 0x7fffffffu, INF_BITS = 0x7f800000u, MINUS_INF = 0xff800000u;
 
+        // Division of numbers below 2^31 by one known to the host: the upper half of a product, shifted.
+        struct fast_divisor
+        {
+            uint32_t by, factor, shift;
+            fast_divisor() = default;
+            explicit fast_divisor(uint32_t d) : by(d), factor(0), shift(0)
+            {
+                while (1ull << (shift + 1) < d)
+                    ++shift;
+                factor = (uint32_t)(((1ull << (32 + shift)) + d - 1) / d); // ceil(2^(32 + shift) / d), 2^shift < d <= 2^(shift + 1)
+            }
+            __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return by == 1 ? n : __umulhi(n, factor) >> shift; }
+        };
+
         struct cache_launch
         {
             aeonb_cache_desc d;
             int              lanes;  // of a group
             int              groups; // of a sequence
+            fast_divisor     by_heads, by_page, by_lanes;
         };
 
         // Where a group's codes and scale lie; -1 for a token without a place.
-        __device__ __forceinline__ int64_t group_place(const aeonb_cache_desc& d, int seq, int token, int head)
+        __device__ __forceinline__ int64_t group_place(const cache_launch& L, int seq, int token, int head)
         {
-            const int64_t at = (int64_t)token + (d.start ? d.start[seq] : 0);
+            const aeonb_cache_desc& d  = L.d;
+            const int64_t           at = (int64_t)token + (d.start ? d.start[seq] : 0);
             if (at < 0 || at >= (int64_t)d.table_pages * d.page_tokens)
                 return -1;
-            const uint32_t page_of = (uint32_t)at / (uint32_t)d.page_tokens; // a position is below 2^32
+            const uint32_t page_of = at < 0x7fffffff ? L.by_page((uint32_t)at) : (uint32_t)at / (uint32_t)d.page_tokens; // (at is below 2^32)
             const int32_t  page    = d.table[seq * d.table_stride + page_of];
             if (page < 0 || page >= d.pages)
                 return -1;
@@ -57,7 +74,8 @@ namespace aeonb
             return s;
         }
 
-        // The code of one value, whatever it is.
+        // The code of one value, whatever it is.  (In 64 bits: numerator and denominator have 24 bits each, so a quotient that is not in the
+        // middle between two codes is at least 2^-25 of it away, and the division's own rounding cannot carry it there.)
         template <int CODE>
         __device__ __noinline__ uint32_t encode_exactly(float x, float scale)
         {
@@ -110,27 +128,80 @@ namespace aeonb
             return r;
         }
 
-        // Codes of four values at once (in the order of the bytes); `exact` is set where one lies too near to a middle to tell.
-        template <int CODE>
-        __device__ __forceinline__ uint32_t encode4(float2 a, float2 b, float inverse, bool& exact)
+        // a b + c for two values at once
+        __device__ __forceinline__ float2 fma2(float2 a, float b, float2 c)
         {
-            const float2 s = mul2(a, inverse), t = mul2(b, inverse);
+            float2 r;
+            asm("{ .reg .b64 t, u, v;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %4};\n"
+                "mov.b64 v, {%5, %6};\n"
+                "fma.rn.f32x2 t, t, u, v;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b), "f"(c.x), "f"(c.y));
+            return r;
+        }
+
+        // x / scale, rounded to nearest.  The remainder t scale - x is exact: t is off by a few units of its last place.  (Taken this way
+        // round, it leaves a zero its sign.)
+        __device__ __forceinline__ float2 quotient2(float2 x, float scale, float inverse)
+        {
+            const float2 t = mul2(x, inverse);
+            return fma2(fma2(t, scale, make_float2(-x.x, -x.y)), -inverse, t);
+        }
+
+        // Codes of four finite values at once (in the order of the bytes).
+        template <int CODE>
+        __device__ __forceinline__ uint32_t encode4(float2 a, float2 b, float scale, float inverse)
+        {
+            float2 s = quotient2(a, scale, inverse), t = quotient2(b, scale, inverse);
             if (CODE == AEONB_CODE_INT8)
             {
-                const float  magic = 12582912.0f; // 1.5 2^23: the sum's last bits are the nearest integer
+                const float  magic = 12582912.0f; // 1.5 2^23: the sum's last bits are the nearest integer, the even one in the middle
                 const float2 up = make_float2(magic, magic), down = make_float2(-magic, -magic);
-                const float2 p = add2(s, up), q = add2(t, up);
-                const float2 r = add2(p, down), u = add2(q, down);
-                const float2 e = add2(s, make_float2(-r.x, -r.y)), f = add2(t, make_float2(-u.x, -u.y));
-                exact |= fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y))) > 0.5f - 0x1p-15f;
+                float2       p = add2(s, up), q = add2(t, up);
+                // what the codes leave: above scale / 2 where the quotient lies on the other side of the middle (exact next to it: then
+                // a multiple of half scale's last place, and below 2^24 of them)
+                const float2 e = fma2(add2(p, down), -scale, a), f = fma2(add2(q, down), -scale, b);
+                const float  half = __fmul_rn(0.5f, scale);
+                if (fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y))) > half)
+                {
+                    p.x = fabsf(e.x) > half ? __fadd_rn(p.x, copysignf(1.0f, e.x)) : p.x;
+                    p.y = fabsf(e.y) > half ? __fadd_rn(p.y, copysignf(1.0f, e.y)) : p.y;
+                    q.x = fabsf(f.x) > half ? __fadd_rn(q.x, copysignf(1.0f, f.x)) : q.x;
+                    q.y = fabsf(f.y) > half ? __fadd_rn(q.y, copysignf(1.0f, f.y)) : q.y;
+                }
                 const uint32_t lo = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040),
                                hi = __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040);
                 return __byte_perm(lo, hi, 0x5410);
             }
-            const float v[4] = {s.x, s.y, t.x, t.y};
+            // a number's bits behind the three that e4m3 keeps are 100... in the middle; below 2^-6 it keeps fewer
+            uint32_t v[4] = {__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(t.x), __float_as_uint(t.y)};
+            const float x[4] = {a.x, a.y, b.x, b.y};
+            uint32_t    off   = 0xffffffffu;
+            float       least = 1.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) // the bits behind the three that a normal e4m3 keeps; below 2^-6 it keeps fewer
-                exact |= (__float_as_uint(v[i]) & 0xfffffu) - 0x7fff8u <= 16u || (fabsf(v[i]) < 0x1p-6f && v[i] != 0.0f);
+            for (int i = 0; i < 4; ++i)
+            {
+                off   = min(off, (v[i] ^ 0x80000u) & 0xfffffu);
+                least = fminf(least, fabsf(__uint_as_float(v[i])));
+            }
+            if (off == 0 || least < 0x1p-6f)
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const float y      = __uint_as_float(v[i]);
+                    const float u      = __fmul_rn(y, 512.0f); // the codes below 2^-6 are multiples of 2^-9
+                    const bool  middle = fabsf(y) < 0x1p-6f ? fabsf(__fsub_rn(u, truncf(u))) == 0.5f : (v[i] & 0xfffffu) == 0x80000u;
+                    const float r      = __fmaf_rn(y, scale, -x[i]); // above 0: the quotient is smaller
+                    if (middle && r != 0.0f)
+                        v[i] += (r > 0.0f) == (y > 0.0f) ? 0xffffffffu : 1u;
+                }
+                s = make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+                t = make_float2(__uint_as_float(v[2]), __uint_as_float(v[3]));
+            }
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
             return lo | hi << 16;
         }
@@ -308,26 +379,36 @@ namespace aeonb
                 }
         }
 
-        // Codes of a chunk, written; the chunk then holds the values that they stand for.
+        // Codes of a chunk, written; the chunk then holds the values that they stand for.  finite: no -infinity in the group; tame: it has a
+        // scale, and that is so large that remainders are exact.
         template <typename T, int CODE, int V>
-        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, float scale, float inverse, bool finite, uint8_t* codes)
+        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, float scale, float inverse, bool finite, bool tame, uint8_t* codes)
         {
+            const bool exact = !tame;
             if constexpr (V == 1)
             {
-                bool     exact = !finite;
-                uint32_t q     = encode4<CODE>(make_float2(x.v, 0.0f), make_float2(0.0f, 0.0f), inverse, exact) & 0xff;
-                if (exact)
+                const bool gone = !finite && __float_as_uint(x.v) == MINUS_INF;
+                uint32_t   q    = encode4<CODE>(make_float2(gone ? 0.0f : x.v, 0.0f), make_float2(0.0f, 0.0f), scale, inverse) & 0xff;
+                if (exact || gone)
                     q = encode_exactly<CODE>(x.v, scale);
                 *codes = (uint8_t)q;
-                x.v              = decode<CODE>(q, scale);
+                x.v    = decode<CODE>(q, scale);
             }
             else
             {
-                uint32_t q[V / 4];
-                bool     exact = !finite;
+                uint32_t q[V / 4], gone = 0; // a bit for each -infinity, which counts as 0 meanwhile
+                if (!finite)
+#pragma unroll
+                    for (int i = 0; i < V / 2; ++i)
+                    {
+                        float2     v = x.pair(i);
+                        const bool a = __float_as_uint(v.x) == MINUS_INF, b = __float_as_uint(v.y) == MINUS_INF;
+                        gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
+                        x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
+                    }
 #pragma unroll
                 for (int i = 0; i < V / 4; ++i)
-                    q[i] = encode4<CODE>(x.pair(2 * i), x.pair(2 * i + 1), inverse, exact);
+                    q[i] = encode4<CODE>(x.pair(2 * i), x.pair(2 * i + 1), scale, inverse);
                 if (exact)
 #pragma unroll
                     for (int i = 0; i < V / 4; ++i)
@@ -336,6 +417,11 @@ namespace aeonb
                         q[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
                                encode_exactly<CODE>(b.y, scale) << 24;
                     }
+                if (gone && scale == scale)
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (gone >> i & 1)
+                            q[i / 4] = (q[i / 4] & ~(0xffu << (8 * (i & 3)))) | (CODE == AEONB_CODE_INT8 ? 0x80u : 0xffu) << (8 * (i & 3));
                 if constexpr (V == 16)
                     *reinterpret_cast<uint4*>(codes) = make_uint4(q[0], q[1], q[2], q[3]);
                 else if constexpr (V == 8)
@@ -346,157 +432,240 @@ namespace aeonb
             }
         }
 
-        // NC chunks a lane; 0: as many as it takes, read a second time for their codes.
-        template <typename T, int CODE, int V, int NC>
+        // Where a lane finds its group: `at_once` groups of L.lanes lanes in a warp, U of them in turn, a block's width apart.
+        struct spot
+        {
+            int l, base, first, apart;
+            bool used;
+            __device__ __forceinline__ spot(const cache_launch& L, int turns)
+            {
+                const int lane = threadIdx.x & 31, at_once = (int)L.by_lanes(32), mine = (int)L.by_lanes((uint32_t)lane);
+                base  = mine * L.lanes;
+                l     = lane - base;
+                used  = mine < at_once;
+                apart = (int)(blockDim.x / 32) * at_once;
+                first = (int)blockIdx.x * apart * turns + (int)(threadIdx.x / 32) * at_once + mine;
+            }
+        };
+
+        template <typename T>
+        __device__ __forceinline__ T* group_rows(void* p, int seq, int token, int head, int64_t by_seq, int64_t by_token, int64_t by_head)
+        {
+            return static_cast<T*>(p) + seq * by_seq + token * by_token + head * by_head;
+        }
+
+        // NC chunks a lane, U groups in turn; NC = 0: as many chunks as it takes, read a second time for their codes.
+        template <typename T, int CODE, int V, int NC, int U>
         __global__ void __launch_bounds__(256) cache_write_kernel(const cache_launch L)
         {
             const aeonb_cache_desc& d      = L.d;
-            const int               lane   = threadIdx.x & 31, mine = lane / L.lanes, base = mine * L.lanes, l = lane - base, at_once = 32 / L.lanes;
-            const int               group  = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * at_once + mine;
-            const int               token  = (uint32_t)group / (uint32_t)d.heads, head = group - token * d.heads;
+            const spot              at(L, U);
             const int               chunks = d.dim / V;
             for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
-                const bool    there = mine < at_once && group < L.groups && token < tokens_of(d, seq);
-                const int64_t place = there ? group_place(d, seq, token, head) : -1;
-                if (there && place < 0 && l == 0 && d.status)
-                    *d.status = 1;
-                const T*    x = static_cast<const T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
-                chunk<T, V> c[NC ? NC : 1];
-                uint32_t    m = 0;
-                if (place >= 0)
-                {
-                    if constexpr (NC > 0)
-                    {
+                const int tokens = tokens_of(d, seq);
+                if ((int)L.by_heads((uint32_t)(blockIdx.x * at.apart * U)) >= tokens)
+                    continue; // the block's first token lies behind the sequence
+                chunk<T, V> c[U][NC ? NC : 1];
+                int64_t     place[U];
+                int         token[U], head[U];
+                uint32_t    m[U];
 #pragma unroll
-                        for (int j = 0; j < NC; ++j)
-                            if (j * L.lanes + l < chunks)
-                            {
-                                c[j].load(x + (j * L.lanes + l) * V);
-                                m = max(m, c[j].largest());
-                            }
-                    }
-                    else
-                        for (int i = l; i < chunks; i += L.lanes)
-                        {
-                            c[0].load(x + (int64_t)i * V);
-                            m = max(m, c[0].largest());
-                        }
-                }
-                m                 = group_largest(m, L.lanes, base, l);
-                const bool finite = m < INF_BITS;
-                if (__any_sync(0xffffffffu, !finite))
+                for (int u = 0; u < U; ++u)
                 {
-                    // an infinity or NaN somewhere in the warp: the largest without -infinity
-                    uint32_t   n   = 0;
-                    const auto see = [&](float v) {
-                        if (__float_as_uint(v) != MINUS_INF)
-                            n = max(n, __float_as_uint(v) & ABS_BITS);
-                    };
-                    if (place >= 0)
+                    const int group = at.first + u * at.apart;
+                    token[u] = (int)L.by_heads((uint32_t)group);
+                    head[u]  = group - token[u] * d.heads;
+                    m[u]     = 0;
+                    const bool there = at.used && group < L.groups && token[u] < tokens;
+                    const T*   x     = group_rows<T>(d.rows, seq, token[u], head[u], d.row_stride_seq, d.row_stride_token, d.row_stride_head);
+                    if constexpr (NC > 0)
+                        if (there)
+                        {
+#pragma unroll
+                            for (int j = 0; j < NC; ++j)
+                                if (j * L.lanes + at.l < chunks)
+                                    c[u][j].load(x + (j * L.lanes + at.l) * V);
+                        }
+                    place[u] = there ? group_place(L, seq, token[u], head[u]) : -1;
+                    if (there && place[u] < 0 && at.l == 0 && d.status)
+                        *d.status = 1;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                {
+                    const T* x = group_rows<T>(d.rows, seq, token[u], head[u], d.row_stride_seq, d.row_stride_token, d.row_stride_head);
+                    if (place[u] >= 0)
                     {
                         if constexpr (NC > 0)
                         {
 #pragma unroll
                             for (int j = 0; j < NC; ++j)
-                                if (j * L.lanes + l < chunks)
-#pragma unroll
-                                    for (int i = 0; i < V; ++i)
-                                        see(c[j].value(i));
+                                if (j * L.lanes + at.l < chunks)
+                                    m[u] = max(m[u], c[u][j].largest());
                         }
                         else
-                            for (int64_t i = l; i < d.dim; i += L.lanes)
-                                see(to_float(x[i]));
+                            for (int i = at.l; i < chunks; i += L.lanes)
+                            {
+                                c[u][0].load(x + (int64_t)i * V);
+                                m[u] = max(m[u], c[u][0].largest());
+                            }
                     }
-                    m = group_largest(n, L.lanes, base, l);
-                }
-                if (place < 0)
-                    continue;
-                const float scale = group_scale<CODE>(m), inverse = __frcp_rn(scale);
-                if (l == 0)
-                    d.scales[place] = scale;
-                uint8_t* codes = static_cast<uint8_t*>(d.codes) + place * d.dim;
-                T*       v     = d.values ? static_cast<T*>(d.values) + seq * d.value_stride_seq + token * d.value_stride_token + head * d.value_stride_head
-                                          : nullptr;
-                if constexpr (NC > 0)
-                {
-#pragma unroll
-                    for (int j = 0; j < NC; ++j)
-                        if (j * L.lanes + l < chunks)
+                    m[u]              = group_largest(m[u], L.lanes, at.base, at.l);
+                    const bool finite = m[u] < INF_BITS;
+                    if (__any_sync(0xffffffffu, !finite))
+                    {
+                        // an infinity or NaN somewhere in the warp: the largest without -infinity
+                        uint32_t   n   = 0;
+                        const auto see = [&](float v) {
+                            if (__float_as_uint(v) != MINUS_INF)
+                                n = max(n, __float_as_uint(v) & ABS_BITS);
+                        };
+                        if (place[u] >= 0)
                         {
-                            const int at = (j * L.lanes + l) * V;
-                            encode_chunk<T, CODE, V>(c[j], scale, inverse, finite, codes + at);
-                            if (v)
-                                c[j].store(v + at);
+                            if constexpr (NC > 0)
+                            {
+#pragma unroll
+                                for (int j = 0; j < NC; ++j)
+                                    if (j * L.lanes + at.l < chunks)
+#pragma unroll
+                                        for (int i = 0; i < V; ++i)
+                                            see(c[u][j].value(i));
+                            }
+                            else
+                                for (int64_t i = at.l; i < d.dim; i += L.lanes)
+                                    see(to_float(x[i]));
+                        }
+                        m[u] = group_largest(n, L.lanes, at.base, at.l);
+                    }
+                    if (place[u] < 0)
+                        continue;
+                    const float scale = group_scale<CODE>(m[u]), inverse = __frcp_rn(scale);
+                    const bool  tame  = scale > 0x1p-90f || m[u] == 0;
+                    if (at.l == 0)
+                        d.scales[place[u]] = scale;
+                    uint8_t* codes = static_cast<uint8_t*>(d.codes) + place[u] * d.dim;
+                    T*       v     = group_rows<T>(d.values, seq, token[u], head[u], d.value_stride_seq, d.value_stride_token, d.value_stride_head);
+                    if constexpr (NC > 0)
+                    {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            if (j * L.lanes + at.l < chunks)
+                            {
+                                const int i = (j * L.lanes + at.l) * V;
+                                encode_chunk<T, CODE, V>(c[u][j], scale, inverse, finite, tame, codes + i);
+                                if (d.values)
+                                    c[u][j].store(v + i);
+                            }
+                    }
+                    else
+                        for (int i = at.l; i < chunks; i += L.lanes)
+                        {
+                            c[u][0].load(x + (int64_t)i * V);
+                            encode_chunk<T, CODE, V>(c[u][0], scale, inverse, finite, tame, codes + (int64_t)i * V);
+                            if (d.values)
+                                c[u][0].store(v + (int64_t)i * V);
                         }
                 }
-                else
-                    for (int i = l; i < chunks; i += L.lanes)
-                    {
-                        const int64_t at = (int64_t)i * V;
-                        c[0].load(x + at);
-                        encode_chunk<T, CODE, V>(c[0], scale, inverse, finite, codes + at);
-                        if (v)
-                            c[0].store(v + at);
-                    }
             }
         }
 
-        template <typename T, int CODE, int V>
+        template <int V>
+        struct code_words
+        {
+            uint32_t w[V / 4 ? V / 4 : 1];
+            __device__ __forceinline__ void load(const uint8_t* q)
+            {
+                if constexpr (V == 16)
+                {
+                    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(q));
+                    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                }
+                else if constexpr (V == 8)
+                {
+                    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(q));
+                    w[0] = u.x, w[1] = u.y;
+                }
+                else if constexpr (V == 4)
+                    w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
+                else
+                    w[0] = *q;
+            }
+        };
+
+        template <typename T, int CODE, int V, int NC, int U>
         __global__ void __launch_bounds__(256) cache_read_kernel(const cache_launch L)
         {
-            const aeonb_cache_desc& d     = L.d;
-            const int               lane  = threadIdx.x & 31, mine = lane / L.lanes, l = lane - mine * L.lanes, at_once = 32 / L.lanes;
-            const int               group = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * at_once + mine;
-            const int               token = (uint32_t)group / (uint32_t)d.heads, head = group - token * d.heads;
+            const aeonb_cache_desc& d = L.d;
+            const spot              at(L, U);
             const int               chunks = d.dim / V;
-            if (mine >= at_once || group >= L.groups)
+            if (!at.used)
                 return;
             for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
-                T*          v = static_cast<T*>(d.rows) + seq * d.row_stride_seq + token * d.row_stride_token + head * d.row_stride_head;
-                chunk<T, V> c;
-                int64_t     place = -1;
-                if (token < tokens_of(d, seq))
+                const int     tokens = tokens_of(d, seq);
+                code_words<V> q[U][NC ? NC : 1];
+                float         scale[U];
+                const uint8_t* codes[U];
+                T*            v[U];
+                bool          given[U]; // codes stand for the group's values (else the scale itself does: 0 or NaN)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
                 {
-                    place = group_place(d, seq, token, head);
-                    c.fill(__uint_as_float(0x7fffffffu));
-                    if (place < 0 && l == 0 && d.status)
-                        *d.status = 1;
-                }
-                else
-                    c.fill(0.0f);
-                if (place < 0)
-                {
-                    for (int i = l; i < chunks; i += L.lanes)
-                        c.store(v + (int64_t)i * V);
-                    continue;
-                }
-                const float    scale = d.scales[place];
-                const uint8_t* codes = static_cast<const uint8_t*>(d.codes) + place * d.dim;
-                for (int i = l; i < chunks; i += L.lanes)
-                {
-                    const uint8_t* q = codes + (int64_t)i * V;
-                    if constexpr (V == 1)
-                        c.v = decode<CODE>(*q, scale);
-                    else
+                    const int group = at.first + u * at.apart, token = (int)L.by_heads((uint32_t)group), head = group - token * d.heads;
+                    int64_t   place = -1;
+                    v[u]     = group < L.groups ? group_rows<T>(d.rows, seq, token, head, d.row_stride_seq, d.row_stride_token, d.row_stride_head) : nullptr;
+                    scale[u] = 0.0f;
+                    if (v[u] && token < tokens)
                     {
-                        uint32_t w[V / 4];
-                        if constexpr (V == 16)
-                        {
-                            const uint4 u = __ldcs(reinterpret_cast<const uint4*>(q));
-                            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-                        }
-                        else if constexpr (V == 8)
-                        {
-                            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(q));
-                            w[0] = u.x, w[1] = u.y;
-                        }
-                        else
-                            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
-                        decode_words<T, CODE, V>(c, w, scale);
+                        place    = group_place(L, seq, token, head);
+                        scale[u] = __uint_as_float(0x7fffffffu);
+                        if (place < 0 && at.l == 0 && d.status)
+                            *d.status = 1;
                     }
-                    c.store(v + (int64_t)i * V);
+                    given[u] = place >= 0;
+                    codes[u] = static_cast<const uint8_t*>(d.codes) + place * d.dim;
+                    if (given[u])
+                    {
+                        scale[u] = d.scales[place];
+                        if constexpr (NC > 0)
+                        {
+#pragma unroll
+                            for (int j = 0; j < NC; ++j)
+                                if (j * L.lanes + at.l < chunks)
+                                    q[u][j].load(codes[u] + (j * L.lanes + at.l) * V);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                {
+                    if (!v[u])
+                        continue;
+                    const auto put = [&](code_words<V>& w, int i) {
+                        chunk<T, V> c;
+                        if (!given[u])
+                            c.fill(scale[u]);
+                        else if constexpr (V == 1)
+                            c.v = decode<CODE>(w.w[0], scale[u]);
+                        else
+                            decode_words<T, CODE, V>(c, w.w, scale[u]);
+                        c.store(v[u] + (int64_t)i * V);
+                    };
+                    if constexpr (NC > 0)
+                    {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            if (j * L.lanes + at.l < chunks)
+                                put(q[u][j], j * L.lanes + at.l);
+                    }
+                    else
+                        for (int i = at.l; i < chunks; i += L.lanes)
+                        {
+                            if (given[u])
+                                q[u][0].load(codes[u] + (int64_t)i * V);
+                            put(q[u][0], i);
+                        }
                 }
             }
         }
@@ -551,22 +720,42 @@ namespace aeonb
                 throw std::invalid_argument("negative stride");
         }
 
+        template <typename T, int CODE, int V, int NC, int U>
+        void launch_lanes(cache_launch& L, bool write, cudaStream_t stream)
+        {
+            const int chunks  = L.d.dim / V;
+            L.lanes           = NC ? (chunks + NC - 1) / NC : 32;
+            L.by_lanes        = fast_divisor(L.lanes);
+            const int at_once = 32 / L.lanes;
+            const int warps   = (int)std::min<int64_t>(8, ((int64_t)L.groups + at_once - 1) / at_once);
+            const int each    = warps * at_once * U;
+            const dim3 grid((unsigned)(((int64_t)L.groups + each - 1) / each), (unsigned)std::min(L.d.seqs, 65535));
+            if (write)
+                cache_write_kernel<T, CODE, V, NC, U><<<grid, warps * 32, 0, stream>>>(L);
+            else
+                cache_read_kernel<T, CODE, V, NC, U><<<grid, warps * 32, 0, stream>>>(L);
+        }
+
         template <typename T, int CODE, int V>
         void launch_chunks(cache_launch& L, bool write, cudaStream_t stream)
         {
             const int chunks = L.d.dim / V;
-            L.lanes          = std::min(chunks, 32);
-            const int warps  = (int)std::min<int64_t>(8, ((int64_t)L.groups + 32 / L.lanes - 1) / (32 / L.lanes));
-            const int each   = warps * (32 / L.lanes);
-            const dim3 grid((unsigned)(((int64_t)L.groups + each - 1) / each), (unsigned)std::min(L.d.seqs, 65535));
-            if (!write)
-                cache_read_kernel<T, CODE, V><<<grid, warps * 32, 0, stream>>>(L);
-            else if (chunks <= 32)
-                cache_write_kernel<T, CODE, V, 1><<<grid, warps * 32, 0, stream>>>(L);
-            else if (chunks <= 32 * 4)
-                cache_write_kernel<T, CODE, V, 4><<<grid, warps * 32, 0, stream>>>(L);
+            if constexpr (V == 1)
+            {
+                // single values: four or eight a lane, so that what a lane finds out about its group serves more than one
+                if (chunks <= 32 * 4)
+                    return launch_lanes<T, CODE, V, 4, 2>(L, write, stream);
+                if (chunks <= 32 * 8)
+                    return launch_lanes<T, CODE, V, 8, 1>(L, write, stream);
+            }
             else
-                cache_write_kernel<T, CODE, V, 0><<<grid, warps * 32, 0, stream>>>(L);
+            {
+                if (chunks <= 32)
+                    return launch_lanes<T, CODE, V, 1, 2>(L, write, stream);
+                if (chunks <= 32 * 4)
+                    return launch_lanes<T, CODE, V, 4, 1>(L, write, stream);
+            }
+            launch_lanes<T, CODE, V, 0, 1>(L, write, stream);
         }
 
         // bytes that every group's first value lies on
@@ -623,10 +812,14 @@ namespace aeonb
                 check_cache(d, write);
                 if (d.seqs == 0 || d.tokens == 0)
                     return AEONB_OK;
-                if ((int64_t)d.tokens * d.heads > 0x7fffff00)
+                if ((int64_t)d.tokens * d.heads > 0x7ffff000)
                     throw error(AEONB_ERR_UNSUPPORTED, "more tokens and heads of a sequence than a launch takes");
                 device_scope   scope(ctx->device);
-                cache_launch   L{d, 0, d.tokens * d.heads};
+                cache_launch   L{};
+                L.d        = d;
+                L.groups   = d.tokens * d.heads;
+                L.by_heads = fast_divisor(d.heads);
+                L.by_page  = fast_divisor(d.page_tokens);
                 const int64_t  groups = (int64_t)d.seqs * d.tokens * d.heads;
                 const int64_t  values = groups * d.dim;
                 const cudaStream_t stream = d.stream ? static_cast<cudaStream_t>(d.stream) : ctx->stream;
