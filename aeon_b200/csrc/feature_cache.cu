@@ -4,10 +4,9 @@
 // else one value; several groups share a warp.  Its largest magnitude is that of the bit patterns without their sign; only where
 // that is no finite number are infinities looked at one by one.  Floor: the bytes of rows, codes and scales.
 //
-// Codes are those of the exact quotient x / scale.  It is formed as x times the reciprocal and corrected by its own remainder once, which
-// gives the quotient of 24 bits; one in the middle between two codes then is exactly there and goes to the even code.  What remains
-// is a quotient that is only rounded to the middle (often so in 16-bit rows, whose values and largest value are ratios of small
-// numbers, but for the rounding of the scale): the sign of the remainder behind it tells on which side it lies.
+// Codes are those of the exact quotient x / scale, which is formed rounded to odd: cut to 24 bits, with the last one set where something was
+// cut.  A code keeps far fewer bits, so it rounds from there as it would from the quotient itself (16-bit rows are full of quotients
+// next to the middle between two codes: ratios of small numbers, but for the rounding of the scale).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -128,7 +127,7 @@ namespace aeonb
             return r;
         }
 
-        // a b + c for two values at once
+        // a b + c for two values at once, to nearest and cut
         __device__ __forceinline__ float2 fma2(float2 a, float b, float2 c)
         {
             float2 r;
@@ -142,68 +141,64 @@ namespace aeonb
                 : "f"(a.x), "f"(a.y), "f"(b), "f"(c.x), "f"(c.y));
             return r;
         }
-
-        // x / scale, rounded to nearest.  The remainder t scale - x is exact: t is off by a few units of its last place.  (Taken this way
-        // round, it leaves a zero its sign.)
-        __device__ __forceinline__ float2 quotient2(float2 x, float scale, float inverse)
+        __device__ __forceinline__ float2 fma2_cut(float2 a, float b, float2 c)
         {
-            const float2 t = mul2(x, inverse);
-            return fma2(fma2(t, scale, make_float2(-x.x, -x.y)), -inverse, t);
+            float2 r;
+            asm("{ .reg .b64 t, u, v;\n"
+                "mov.b64 t, {%2, %3};\n"
+                "mov.b64 u, {%4, %4};\n"
+                "mov.b64 v, {%5, %6};\n"
+                "fma.rz.f32x2 t, t, u, v;\n"
+                "mov.b64 {%0, %1}, t; }"
+                : "=f"(r.x), "=f"(r.y)
+                : "f"(a.x), "f"(a.y), "f"(b), "f"(c.x), "f"(c.y));
+            return r;
         }
 
-        // Codes of four finite values at once (in the order of the bytes).
-        template <int CODE>
-        __device__ __forceinline__ uint32_t encode4(float2 a, float2 b, float scale, float inverse)
+        // What a group's values are divided with: minus the reciprocal of the scale, a little too small and a little too large (by three and
+        // by four units of the last place of its nearest float).
+        struct divisor
         {
-            float2 s = quotient2(a, scale, inverse), t = quotient2(b, scale, inverse);
+            float scale, small, large;
+            __device__ __forceinline__ explicit divisor(float s) : scale(s)
+            {
+                const uint32_t inverse = __float_as_uint(__frcp_rn(s));
+                small                  = -__uint_as_float(inverse - 3);
+                large                  = -__uint_as_float(inverse + 4);
+            }
+        };
+
+        // -x / scale for two values, rounded to odd.  The first guess t is not above the quotient q (in magnitude), five units of its last
+        // place below it at most; the correction by its remainder, a little too large (2^-20 of those units at most), ends at q or
+        // just above and is cut, so a q of 24 bits comes out itself and another one cut (none lies that close below a float: q has a
+        // numerator and denominator of 24 bits).  The second remainder, exact again, is 0 for the former only.  (Of this sign, the
+        // steps leave a zero's sign as it should be.)
+        __device__ __forceinline__ float2 minus_quotient2(float2 x, const divisor& by)
+        {
+            const float2 t = mul2(x, by.small);
+            const float2 y = fma2_cut(fma2(t, by.scale, x), by.large, t);
+            const float2 r = fma2(y, by.scale, x);
+            return make_float2(__uint_as_float(__float_as_uint(y.x) | (r.x != 0.0f ? 1u : 0u)),
+                               __uint_as_float(__float_as_uint(y.y) | (r.y != 0.0f ? 1u : 0u)));
+        }
+
+        // Codes of four finite values at once (in the order of the bytes); for int8 the values become the codes' numbers.
+        template <int CODE>
+        __device__ __forceinline__ uint32_t encode4(float2& a, float2& b, const divisor& by)
+        {
+            const float2 s = minus_quotient2(a, by), t = minus_quotient2(b, by);
             if (CODE == AEONB_CODE_INT8)
             {
-                const float  magic = 12582912.0f; // 1.5 2^23: the sum's last bits are the nearest integer, the even one in the middle
+                const float  magic = 12582912.0f; // 1.5 2^23: the difference's last bits are the nearest integer, the even one in the middle
                 const float2 up = make_float2(magic, magic), down = make_float2(-magic, -magic);
-                float2       p = add2(s, up), q = add2(t, up);
-                // what the codes leave: above scale / 2 where the quotient lies on the other side of the middle (exact next to it: then
-                // a multiple of half scale's last place, and below 2^24 of them)
-                const float2 e = fma2(add2(p, down), -scale, a), f = fma2(add2(q, down), -scale, b);
-                const float  half = __fmul_rn(0.5f, scale);
-                if (fmaxf(fmaxf(fabsf(e.x), fabsf(e.y)), fmaxf(fabsf(f.x), fabsf(f.y))) > half)
-                {
-                    p.x = fabsf(e.x) > half ? __fadd_rn(p.x, copysignf(1.0f, e.x)) : p.x;
-                    p.y = fabsf(e.y) > half ? __fadd_rn(p.y, copysignf(1.0f, e.y)) : p.y;
-                    q.x = fabsf(f.x) > half ? __fadd_rn(q.x, copysignf(1.0f, f.x)) : q.x;
-                    q.y = fabsf(f.y) > half ? __fadd_rn(q.y, copysignf(1.0f, f.y)) : q.y;
-                }
+                const float2 p = fma2(s, -1.0f, up), q = fma2(t, -1.0f, up);
+                a = add2(p, down), b = add2(q, down);
                 const uint32_t lo = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040),
                                hi = __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040);
                 return __byte_perm(lo, hi, 0x5410);
             }
-            // a number's bits behind the three that e4m3 keeps are 100... in the middle; below 2^-6 it keeps fewer
-            uint32_t v[4] = {__float_as_uint(s.x), __float_as_uint(s.y), __float_as_uint(t.x), __float_as_uint(t.y)};
-            const float x[4] = {a.x, a.y, b.x, b.y};
-            uint32_t    off   = 0xffffffffu;
-            float       least = 1.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                off   = min(off, (v[i] ^ 0x80000u) & 0xfffffu);
-                least = fminf(least, fabsf(__uint_as_float(v[i])));
-            }
-            if (off == 0 || least < 0x1p-6f)
-            {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                {
-                    const float y      = __uint_as_float(v[i]);
-                    const float u      = __fmul_rn(y, 512.0f); // the codes below 2^-6 are multiples of 2^-9
-                    const bool  middle = fabsf(y) < 0x1p-6f ? fabsf(__fsub_rn(u, truncf(u))) == 0.5f : (v[i] & 0xfffffu) == 0x80000u;
-                    const float r      = __fmaf_rn(y, scale, -x[i]); // above 0: the quotient is smaller
-                    if (middle && r != 0.0f)
-                        v[i] += (r > 0.0f) == (y > 0.0f) ? 0xffffffffu : 1u;
-                }
-                s = make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
-                t = make_float2(__uint_as_float(v[2]), __uint_as_float(v[3]));
-            }
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3);
-            return lo | hi << 16;
+            return (lo | hi << 16) ^ 0x80808080u;
         }
 
         // Whether one of four codes stands for no finite number.
@@ -379,17 +374,18 @@ namespace aeonb
                 }
         }
 
-        // Codes of a chunk, written; the chunk then holds the values that they stand for.  finite: no -infinity in the group; tame: it has a
-        // scale, and that is so large that remainders are exact.
+        // Codes of a chunk, written; with `values` the chunk then holds the values that they stand for.  finite: no -infinity in the group;
+        // tame: it has a scale, and that is so large that remainders are exact.
         template <typename T, int CODE, int V>
-        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, float scale, float inverse, bool finite, bool tame, uint8_t* codes)
+        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, const divisor& by, bool finite, bool tame, uint8_t* codes, bool values)
         {
-            const bool exact = !tame;
+            const float scale = by.scale;
             if constexpr (V == 1)
             {
                 const bool gone = !finite && __float_as_uint(x.v) == MINUS_INF;
-                uint32_t   q    = encode4<CODE>(make_float2(gone ? 0.0f : x.v, 0.0f), make_float2(0.0f, 0.0f), scale, inverse) & 0xff;
-                if (exact || gone)
+                float2     v = make_float2(gone ? 0.0f : x.v, 0.0f), none = make_float2(0.0f, 0.0f);
+                uint32_t   q = encode4<CODE>(v, none, by) & 0xff;
+                if (!tame || gone)
                     q = encode_exactly<CODE>(x.v, scale);
                 *codes = (uint8_t)q;
                 x.v    = decode<CODE>(q, scale);
@@ -406,10 +402,24 @@ namespace aeonb
                         gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
                         x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
                     }
+                if (tame)
+                {
 #pragma unroll
-                for (int i = 0; i < V / 4; ++i)
-                    q[i] = encode4<CODE>(x.pair(2 * i), x.pair(2 * i + 1), scale, inverse);
-                if (exact)
+                    for (int i = 0; i < V / 4; ++i)
+                    {
+                        float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
+                        q[i] = encode4<CODE>(a, b, by);
+                        if (values)
+                        {
+                            if (CODE != AEONB_CODE_INT8)
+                                numbers4<CODE>(q[i], a, b);
+                            x.set(2 * i, mul2(a, scale));
+                            x.set(2 * i + 1, mul2(b, scale));
+                        }
+                    }
+                }
+                else
+                {
 #pragma unroll
                     for (int i = 0; i < V / 4; ++i)
                     {
@@ -417,18 +427,22 @@ namespace aeonb
                         q[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
                                encode_exactly<CODE>(b.y, scale) << 24;
                     }
+                    decode_words<T, CODE, V>(x, q, scale);
+                }
                 if (gone && scale == scale)
+                {
 #pragma unroll
                     for (int i = 0; i < V; ++i)
                         if (gone >> i & 1)
                             q[i / 4] = (q[i / 4] & ~(0xffu << (8 * (i & 3)))) | (CODE == AEONB_CODE_INT8 ? 0x80u : 0xffu) << (8 * (i & 3));
+                    decode_words<T, CODE, V>(x, q, scale);
+                }
                 if constexpr (V == 16)
                     *reinterpret_cast<uint4*>(codes) = make_uint4(q[0], q[1], q[2], q[3]);
                 else if constexpr (V == 8)
                     *reinterpret_cast<uint2*>(codes) = make_uint2(q[0], q[1]);
                 else
                     *reinterpret_cast<uint32_t*>(codes) = q[0];
-                decode_words<T, CODE, V>(x, q, scale);
             }
         }
 
@@ -456,7 +470,7 @@ namespace aeonb
 
         // NC chunks a lane, U groups in turn; NC = 0: as many chunks as it takes, read a second time for their codes.
         template <typename T, int CODE, int V, int NC, int U>
-        __global__ void __launch_bounds__(256) cache_write_kernel(const cache_launch L)
+        __global__ void __launch_bounds__(256, 4) cache_write_kernel(const cache_launch L)
         {
             const aeonb_cache_desc& d      = L.d;
             const spot              at(L, U);
@@ -540,7 +554,8 @@ namespace aeonb
                     }
                     if (place[u] < 0)
                         continue;
-                    const float scale = group_scale<CODE>(m[u]), inverse = __frcp_rn(scale);
+                    const float   scale = group_scale<CODE>(m[u]);
+                    const divisor by(scale);
                     const bool  tame  = scale > 0x1p-90f || m[u] == 0;
                     if (at.l == 0)
                         d.scales[place[u]] = scale;
@@ -553,7 +568,7 @@ namespace aeonb
                             if (j * L.lanes + at.l < chunks)
                             {
                                 const int i = (j * L.lanes + at.l) * V;
-                                encode_chunk<T, CODE, V>(c[u][j], scale, inverse, finite, tame, codes + i);
+                                encode_chunk<T, CODE, V>(c[u][j], by, finite, tame, codes + i, d.values != nullptr);
                                 if (d.values)
                                     c[u][j].store(v + i);
                             }
@@ -562,7 +577,7 @@ namespace aeonb
                         for (int i = at.l; i < chunks; i += L.lanes)
                         {
                             c[u][0].load(x + (int64_t)i * V);
-                            encode_chunk<T, CODE, V>(c[u][0], scale, inverse, finite, tame, codes + (int64_t)i * V);
+                            encode_chunk<T, CODE, V>(c[u][0], by, finite, tame, codes + (int64_t)i * V, d.values != nullptr);
                             if (d.values)
                                 c[u][0].store(v + (int64_t)i * V);
                         }
@@ -750,8 +765,11 @@ namespace aeonb
             }
             else
             {
-                if (chunks <= 32)
-                    return launch_lanes<T, CODE, V, 1, 2>(L, write, stream);
+                // Two chunks a lane: what a lane finds out about its group serves both.  64 x 4096 x 8 groups of 128 bf16 to int8 with values,
+                // one chunk and two groups in turn / two chunks / four: 0.33 / 0.26 / 0.26 ms; e4m3 0.38 / 0.32 / 0.34; groups of 64 floats
+                // 0.24 / 0.19 / 0.22; read back 0.14 / 0.13 / 0.13.
+                if (chunks <= 32 * 2)
+                    return launch_lanes<T, CODE, V, 2, 1>(L, write, stream);
                 if (chunks <= 32 * 4)
                     return launch_lanes<T, CODE, V, 4, 1>(L, write, stream);
             }
