@@ -1,7 +1,7 @@
 // The feature cache on sm_100a: rows of floats to 8-bit codes in pages, with a scale for each token and head, and back.
 //
-// A group (token and head) is read once: up to 32 lanes hold a chunk each, of 32 bytes of the rows where their place allows it, else 16,
-// else one value; several groups share a warp.  Its largest magnitude is that of the bit patterns without their sign; only where
+// A group (token and head) is read once: up to 32 lanes hold chunks of it, of 32 bytes of the rows where their place allows it, else 16,
+// else four values that lie the group's lanes apart; several groups share a warp.  Its largest magnitude is that of the bit patterns without their sign; only where
 // that is no finite number are infinities looked at one by one.  Floor: the bytes of rows, codes and scales.
 //
 // Codes are those of the exact quotient x / scale, which is formed rounded to odd: cut to 24 bits, with the last one set where something was
@@ -229,14 +229,17 @@ namespace aeonb
             b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
         }
 
-        // V values of a row in one lane's registers, and how they get there and away.
+        // V values of a row in one lane's registers, and how they and their codes get there and away.  `step` and `left` are for values apart:
+        // how far they lie from one another, and how many of the group's come from the chunk's first one on.
         template <typename T, int V>
         struct chunk
         {
-            static constexpr int  W    = V * sizeof(T) / 4; // words
+            static constexpr int  N = V, W = V * sizeof(T) / 4; // values, words
             static constexpr bool WIDE = sizeof(T) == 4;
             uint32_t              w[W];
-            __device__ __forceinline__ void load(const T* p)
+            // where lane l of L finds its chunk j
+            __device__ __forceinline__ static int place(int j, int l, int L) { return (j * L + l) * V; }
+            __device__ __forceinline__ void load(const T* p, int, int)
             {
                 if constexpr (W == 8)
                     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -249,7 +252,7 @@ namespace aeonb
                     w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
                 }
             }
-            __device__ __forceinline__ void store(T* p) const
+            __device__ __forceinline__ void store(T* p, int, int) const
             {
                 if constexpr (W == 8)
                     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
@@ -325,16 +328,81 @@ namespace aeonb
             }
         };
 
-        // One value: rows that lie on no 16 bytes.
+        // Four values apart: rows that lie on no 16 bytes.
+        constexpr int APART = -4;
         template <typename T>
-        struct chunk<T, 1>
+        struct chunk<T, APART>
         {
-            float v;
-            __device__ __forceinline__ void     load(const T* p) { v = to_float(*p); }
-            __device__ __forceinline__ void     store(T* p) const { *p = from_float<T>(v); }
-            __device__ __forceinline__ void     fill(float x) { v = x; }
-            __device__ __forceinline__ uint32_t largest() const { return __float_as_uint(v) & ABS_BITS; }
-            __device__ __forceinline__ float    value(int) const { return v; }
+            static constexpr int N = 4;
+            float                v[4];
+            __device__ __forceinline__ static int place(int j, int l, int L) { return j * 4 * L + l; }
+            __device__ __forceinline__ void       load(const T* p, int step, int left)
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = i * step < left ? to_float(p[i * step]) : 0.0f;
+            }
+            __device__ __forceinline__ void store(T* p, int step, int left) const
+            {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i * step < left)
+                        p[i * step] = from_float<T>(v[i]);
+            }
+            __device__ __forceinline__ void     fill(float x) { v[0] = v[1] = v[2] = v[3] = x; }
+            __device__ __forceinline__ float2   pair(int i) const { return make_float2(v[2 * i], v[2 * i + 1]); }
+            __device__ __forceinline__ void     set(int i, float2 x) { v[2 * i] = x.x, v[2 * i + 1] = x.y; }
+            __device__ __forceinline__ float    value(int i) const { return v[i]; }
+            __device__ __forceinline__ uint32_t largest() const
+            {
+                return max(max(__float_as_uint(v[0]) & ABS_BITS, __float_as_uint(v[1]) & ABS_BITS),
+                           max(__float_as_uint(v[2]) & ABS_BITS, __float_as_uint(v[3]) & ABS_BITS));
+            }
+        };
+
+        // The codes of a chunk.
+        template <int V>
+        struct code_words
+        {
+            static constexpr int N = V == APART ? 4 : V;
+            uint32_t             w[N / 4];
+            __device__ __forceinline__ void load(const uint8_t* q, int step, int left)
+            {
+                if constexpr (V == 16)
+                {
+                    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(q));
+                    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+                }
+                else if constexpr (V == 8)
+                {
+                    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(q));
+                    w[0] = u.x, w[1] = u.y;
+                }
+                else if constexpr (V == 4)
+                    w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
+                else
+                {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        b[i] = i * step < left ? q[i * step] : 0;
+                    w[0] = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+                }
+            }
+            __device__ __forceinline__ void store(uint8_t* q, int step, int left) const
+            {
+                if constexpr (V == 16)
+                    *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+                else if constexpr (V == 8)
+                    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+                else if constexpr (V == 4)
+                    *reinterpret_cast<uint32_t*>(q) = w[0];
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i * step < left)
+                            q[i * step] = (uint8_t)(w[0] >> (8 * i));
+            }
         };
 
         // The largest magnitude among a group's lanes, L of them from lane `base` on (any L: the largest of some values does not
@@ -353,112 +421,94 @@ namespace aeonb
         }
 
         template <typename T, int CODE, int V>
-        __device__ __forceinline__ void decode_words(chunk<T, V>& x, const uint32_t* q, float scale)
+        __device__ __forceinline__ void decode_chunk(chunk<T, V>& x, const code_words<V>& q, float scale)
         {
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < V / 4; ++i)
+            for (int i = 0; i < chunk<T, V>::N / 4; ++i)
             {
                 float2 a, b;
-                odd |= odd4<CODE>(q[i]);
-                numbers4<CODE>(q[i], a, b);
+                odd |= odd4<CODE>(q.w[i]);
+                numbers4<CODE>(q.w[i], a, b);
                 x.set(2 * i, mul2(a, scale));
                 x.set(2 * i + 1, mul2(b, scale));
             }
             if (odd)
 #pragma unroll
-                for (int i = 0; i < V / 4; ++i)
+                for (int i = 0; i < chunk<T, V>::N / 4; ++i)
                 {
-                    x.set(2 * i, make_float2(decode<CODE>(q[i] & 0xff, scale), decode<CODE>(q[i] >> 8 & 0xff, scale)));
-                    x.set(2 * i + 1, make_float2(decode<CODE>(q[i] >> 16 & 0xff, scale), decode<CODE>(q[i] >> 24, scale)));
+                    x.set(2 * i, make_float2(decode<CODE>(q.w[i] & 0xff, scale), decode<CODE>(q.w[i] >> 8 & 0xff, scale)));
+                    x.set(2 * i + 1, make_float2(decode<CODE>(q.w[i] >> 16 & 0xff, scale), decode<CODE>(q.w[i] >> 24, scale)));
                 }
         }
 
-        // Codes of a chunk, written; with `values` the chunk then holds the values that they stand for.  finite: no -infinity in the group;
-        // tame: it has a scale, and that is so large that remainders are exact.
+        // Codes of a chunk; with `values` the chunk then holds the values that they stand for.  finite: no -infinity in the group; tame: it
+        // has a scale, and that is so large that remainders are exact.
         template <typename T, int CODE, int V>
-        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, const divisor& by, bool finite, bool tame, uint8_t* codes, bool values)
+        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, code_words<V>& q, const divisor& by, bool finite, bool tame, bool values)
         {
-            const float scale = by.scale;
-            if constexpr (V == 1)
+            constexpr int N     = chunk<T, V>::N;
+            const float   scale = by.scale;
+            uint32_t      gone  = 0; // a bit for each -infinity, which counts as 0 meanwhile
+            if (!finite)
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i)
+                {
+                    const float2 v = x.pair(i);
+                    const bool   a = __float_as_uint(v.x) == MINUS_INF, b = __float_as_uint(v.y) == MINUS_INF;
+                    gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
+                    x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
+                }
+            if (tame)
             {
-                const bool gone = !finite && __float_as_uint(x.v) == MINUS_INF;
-                float2     v = make_float2(gone ? 0.0f : x.v, 0.0f), none = make_float2(0.0f, 0.0f);
-                uint32_t   q = encode4<CODE>(v, none, by) & 0xff;
-                if (!tame || gone)
-                    q = encode_exactly<CODE>(x.v, scale);
-                *codes = (uint8_t)q;
-                x.v    = decode<CODE>(q, scale);
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i)
+                {
+                    float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
+                    q.w[i] = encode4<CODE>(a, b, by);
+                    if (values)
+                    {
+                        if (CODE != AEONB_CODE_INT8)
+                            numbers4<CODE>(q.w[i], a, b);
+                        x.set(2 * i, mul2(a, scale));
+                        x.set(2 * i + 1, mul2(b, scale));
+                    }
+                }
             }
             else
             {
-                uint32_t q[V / 4], gone = 0; // a bit for each -infinity, which counts as 0 meanwhile
-                if (!finite)
 #pragma unroll
-                    for (int i = 0; i < V / 2; ++i)
-                    {
-                        float2     v = x.pair(i);
-                        const bool a = __float_as_uint(v.x) == MINUS_INF, b = __float_as_uint(v.y) == MINUS_INF;
-                        gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
-                        x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
-                    }
-                if (tame)
+                for (int i = 0; i < N / 4; ++i)
                 {
-#pragma unroll
-                    for (int i = 0; i < V / 4; ++i)
-                    {
-                        float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
-                        q[i] = encode4<CODE>(a, b, by);
-                        if (values)
-                        {
-                            if (CODE != AEONB_CODE_INT8)
-                                numbers4<CODE>(q[i], a, b);
-                            x.set(2 * i, mul2(a, scale));
-                            x.set(2 * i + 1, mul2(b, scale));
-                        }
-                    }
+                    const float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
+                    q.w[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
+                             encode_exactly<CODE>(b.y, scale) << 24;
                 }
-                else
-                {
+                decode_chunk<T, CODE, V>(x, q, scale);
+            }
+            if (gone && scale == scale)
+            {
 #pragma unroll
-                    for (int i = 0; i < V / 4; ++i)
-                    {
-                        const float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
-                        q[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
-                               encode_exactly<CODE>(b.y, scale) << 24;
-                    }
-                    decode_words<T, CODE, V>(x, q, scale);
-                }
-                if (gone && scale == scale)
-                {
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (gone >> i & 1)
-                            q[i / 4] = (q[i / 4] & ~(0xffu << (8 * (i & 3)))) | (CODE == AEONB_CODE_INT8 ? 0x80u : 0xffu) << (8 * (i & 3));
-                    decode_words<T, CODE, V>(x, q, scale);
-                }
-                if constexpr (V == 16)
-                    *reinterpret_cast<uint4*>(codes) = make_uint4(q[0], q[1], q[2], q[3]);
-                else if constexpr (V == 8)
-                    *reinterpret_cast<uint2*>(codes) = make_uint2(q[0], q[1]);
-                else
-                    *reinterpret_cast<uint32_t*>(codes) = q[0];
+                for (int i = 0; i < N; ++i)
+                    if (gone >> i & 1)
+                        q.w[i / 4] = (q.w[i / 4] & ~(0xffu << (8 * (i & 3)))) | (CODE == AEONB_CODE_INT8 ? 0x80u : 0xffu) << (8 * (i & 3));
+                decode_chunk<T, CODE, V>(x, q, scale);
             }
         }
 
-        // Where a lane finds its group: `at_once` groups of L.lanes lanes in a warp, U of them in turn, a block's width apart.
+        // Where a lane finds its group: 32 / L.lanes groups in a warp.
         struct spot
         {
-            int l, base, first, apart;
+            int  l, base, group, block_group; // lane of the group, its first lane, its number and that of the block's first one
             bool used;
-            __device__ __forceinline__ spot(const cache_launch& L, int turns)
+            __device__ __forceinline__ explicit spot(const cache_launch& L)
             {
                 const int lane = threadIdx.x & 31, at_once = (int)L.by_lanes(32), mine = (int)L.by_lanes((uint32_t)lane);
-                base  = mine * L.lanes;
-                l     = lane - base;
-                used  = mine < at_once;
-                apart = (int)(blockDim.x / 32) * at_once;
-                first = (int)blockIdx.x * apart * turns + (int)(threadIdx.x / 32) * at_once + mine;
+                base        = mine * L.lanes;
+                l           = lane - base;
+                used        = mine < at_once;
+                block_group = (int)(blockIdx.x * (blockDim.x / 32)) * at_once;
+                group       = block_group + (int)(threadIdx.x / 32) * at_once + mine;
             }
         };
 
@@ -468,220 +518,165 @@ namespace aeonb
             return static_cast<T*>(p) + seq * by_seq + token * by_token + head * by_head;
         }
 
-        // NC chunks a lane, U groups in turn; NC = 0: as many chunks as it takes, read a second time for their codes.
-        template <typename T, int CODE, int V, int NC, int U>
+        // NC chunks a lane; NC = 0: as many as it takes, read a second time for their codes.
+        template <typename T, int CODE, int V, int NC>
         __global__ void __launch_bounds__(256, 4) cache_write_kernel(const cache_launch L)
         {
-            const aeonb_cache_desc& d      = L.d;
-            const spot              at(L, U);
-            const int               chunks = d.dim / V;
+            typedef chunk<T, V>     C;
+            const aeonb_cache_desc& d = L.d;
+            const spot              at(L);
+            const int               token = (int)L.by_heads((uint32_t)at.group), head = at.group - token * d.heads;
             for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
                 const int tokens = tokens_of(d, seq);
-                if ((int)L.by_heads((uint32_t)(blockIdx.x * at.apart * U)) >= tokens)
+                if ((int)L.by_heads((uint32_t)at.block_group) >= tokens)
                     continue; // the block's first token lies behind the sequence
-                chunk<T, V> c[U][NC ? NC : 1];
-                int64_t     place[U];
-                int         token[U], head[U];
-                uint32_t    m[U];
+                const bool there = at.used && at.group < L.groups && token < tokens;
+                const T*   x     = group_rows<T>(d.rows, seq, token, head, d.row_stride_seq, d.row_stride_token, d.row_stride_head);
+                C          c[NC ? NC : 1];
+                if constexpr (NC > 0)
+                    if (there)
+                    {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                        for (int j = 0; j < NC; ++j)
+                            if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                                c[j].load(x + i, L.lanes, d.dim - i);
+                    }
+                const int64_t place = there ? group_place(L, seq, token, head) : -1;
+                if (there && place < 0 && at.l == 0 && d.status)
+                    *d.status = 1;
+                uint32_t m = 0;
+                if (place >= 0)
                 {
-                    const int group = at.first + u * at.apart;
-                    token[u] = (int)L.by_heads((uint32_t)group);
-                    head[u]  = group - token[u] * d.heads;
-                    m[u]     = 0;
-                    const bool there = at.used && group < L.groups && token[u] < tokens;
-                    const T*   x     = group_rows<T>(d.rows, seq, token[u], head[u], d.row_stride_seq, d.row_stride_token, d.row_stride_head);
                     if constexpr (NC > 0)
-                        if (there)
+                    {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            if (C::place(j, at.l, L.lanes) < d.dim)
+                                m = max(m, c[j].largest());
+                    }
+                    else
+                        for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
                         {
-#pragma unroll
-                            for (int j = 0; j < NC; ++j)
-                                if (j * L.lanes + at.l < chunks)
-                                    c[u][j].load(x + (j * L.lanes + at.l) * V);
+                            c[0].load(x + i, L.lanes, d.dim - i);
+                            m = max(m, c[0].largest());
                         }
-                    place[u] = there ? group_place(L, seq, token[u], head[u]) : -1;
-                    if (there && place[u] < 0 && at.l == 0 && d.status)
-                        *d.status = 1;
                 }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
+                m                 = group_largest(m, L.lanes, at.base, at.l);
+                const bool finite = m < INF_BITS;
+                if (__any_sync(0xffffffffu, !finite))
                 {
-                    const T* x = group_rows<T>(d.rows, seq, token[u], head[u], d.row_stride_seq, d.row_stride_token, d.row_stride_head);
-                    if (place[u] >= 0)
+                    // an infinity or NaN somewhere in the warp: the largest without -infinity
+                    uint32_t   n   = 0;
+                    const auto see = [&](float v) {
+                        if (__float_as_uint(v) != MINUS_INF)
+                            n = max(n, __float_as_uint(v) & ABS_BITS);
+                    };
+                    if (place >= 0)
                     {
                         if constexpr (NC > 0)
                         {
 #pragma unroll
                             for (int j = 0; j < NC; ++j)
-                                if (j * L.lanes + at.l < chunks)
-                                    m[u] = max(m[u], c[u][j].largest());
+                                if (C::place(j, at.l, L.lanes) < d.dim)
+#pragma unroll
+                                    for (int i = 0; i < C::N; ++i)
+                                        see(c[j].value(i));
                         }
                         else
-                            for (int i = at.l; i < chunks; i += L.lanes)
-                            {
-                                c[u][0].load(x + (int64_t)i * V);
-                                m[u] = max(m[u], c[u][0].largest());
-                            }
+                            for (int i = at.l; i < d.dim; i += L.lanes)
+                                see(to_float(x[i]));
                     }
-                    m[u]              = group_largest(m[u], L.lanes, at.base, at.l);
-                    const bool finite = m[u] < INF_BITS;
-                    if (__any_sync(0xffffffffu, !finite))
-                    {
-                        // an infinity or NaN somewhere in the warp: the largest without -infinity
-                        uint32_t   n   = 0;
-                        const auto see = [&](float v) {
-                            if (__float_as_uint(v) != MINUS_INF)
-                                n = max(n, __float_as_uint(v) & ABS_BITS);
-                        };
-                        if (place[u] >= 0)
-                        {
-                            if constexpr (NC > 0)
-                            {
-#pragma unroll
-                                for (int j = 0; j < NC; ++j)
-                                    if (j * L.lanes + at.l < chunks)
-#pragma unroll
-                                        for (int i = 0; i < V; ++i)
-                                            see(c[u][j].value(i));
-                            }
-                            else
-                                for (int64_t i = at.l; i < d.dim; i += L.lanes)
-                                    see(to_float(x[i]));
-                        }
-                        m[u] = group_largest(n, L.lanes, at.base, at.l);
-                    }
-                    if (place[u] < 0)
-                        continue;
-                    const float   scale = group_scale<CODE>(m[u]);
-                    const divisor by(scale);
-                    const bool  tame  = scale > 0x1p-90f || m[u] == 0;
-                    if (at.l == 0)
-                        d.scales[place[u]] = scale;
-                    uint8_t* codes = static_cast<uint8_t*>(d.codes) + place[u] * d.dim;
-                    T*       v     = group_rows<T>(d.values, seq, token[u], head[u], d.value_stride_seq, d.value_stride_token, d.value_stride_head);
-                    if constexpr (NC > 0)
-                    {
-#pragma unroll
-                        for (int j = 0; j < NC; ++j)
-                            if (j * L.lanes + at.l < chunks)
-                            {
-                                const int i = (j * L.lanes + at.l) * V;
-                                encode_chunk<T, CODE, V>(c[u][j], by, finite, tame, codes + i, d.values != nullptr);
-                                if (d.values)
-                                    c[u][j].store(v + i);
-                            }
-                    }
-                    else
-                        for (int i = at.l; i < chunks; i += L.lanes)
-                        {
-                            c[u][0].load(x + (int64_t)i * V);
-                            encode_chunk<T, CODE, V>(c[u][0], by, finite, tame, codes + (int64_t)i * V, d.values != nullptr);
-                            if (d.values)
-                                c[u][0].store(v + (int64_t)i * V);
-                        }
+                    m = group_largest(n, L.lanes, at.base, at.l);
                 }
+                if (place < 0)
+                    continue;
+                const float   scale = group_scale<CODE>(m);
+                const divisor by(scale);
+                const bool    tame = scale > 0x1p-90f || m == 0;
+                if (at.l == 0)
+                    d.scales[place] = scale;
+                uint8_t*   codes = static_cast<uint8_t*>(d.codes) + place * d.dim;
+                T*         v     = group_rows<T>(d.values, seq, token, head, d.value_stride_seq, d.value_stride_token, d.value_stride_head);
+                const auto put   = [&](C& x, int i) {
+                    code_words<V> q;
+                    encode_chunk<T, CODE, V>(x, q, by, finite, tame, d.values != nullptr);
+                    q.store(codes + i, L.lanes, d.dim - i);
+                    if (d.values)
+                        x.store(v + i, L.lanes, d.dim - i);
+                };
+                if constexpr (NC > 0)
+                {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+                        if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                            put(c[j], i);
+                }
+                else
+                    for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
+                    {
+                        c[0].load(x + i, L.lanes, d.dim - i);
+                        put(c[0], i);
+                    }
             }
         }
 
-        template <int V>
-        struct code_words
-        {
-            uint32_t w[V / 4 ? V / 4 : 1];
-            __device__ __forceinline__ void load(const uint8_t* q)
-            {
-                if constexpr (V == 16)
-                {
-                    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(q));
-                    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-                }
-                else if constexpr (V == 8)
-                {
-                    const uint2 u = __ldcs(reinterpret_cast<const uint2*>(q));
-                    w[0] = u.x, w[1] = u.y;
-                }
-                else if constexpr (V == 4)
-                    w[0] = __ldcs(reinterpret_cast<const uint32_t*>(q));
-                else
-                    w[0] = *q;
-            }
-        };
-
-        template <typename T, int CODE, int V, int NC, int U>
+        template <typename T, int CODE, int V, int NC>
         __global__ void __launch_bounds__(256) cache_read_kernel(const cache_launch L)
         {
+            typedef chunk<T, V>     C;
             const aeonb_cache_desc& d = L.d;
-            const spot              at(L, U);
-            const int               chunks = d.dim / V;
-            if (!at.used)
+            const spot              at(L);
+            if (!at.used || at.group >= L.groups)
                 return;
+            const int token = (int)L.by_heads((uint32_t)at.group), head = at.group - token * d.heads;
             for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
-                const int     tokens = tokens_of(d, seq);
-                code_words<V> q[U][NC ? NC : 1];
-                float         scale[U];
-                const uint8_t* codes[U];
-                T*            v[U];
-                bool          given[U]; // codes stand for the group's values (else the scale itself does: 0 or NaN)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
+                T*            v = group_rows<T>(d.rows, seq, token, head, d.row_stride_seq, d.row_stride_token, d.row_stride_head);
+                code_words<V> q[NC ? NC : 1];
+                int64_t       place = -1;
+                float         scale = 0.0f; // of the group, or what it is filled with
+                if (token < tokens_of(d, seq))
                 {
-                    const int group = at.first + u * at.apart, token = (int)L.by_heads((uint32_t)group), head = group - token * d.heads;
-                    int64_t   place = -1;
-                    v[u]     = group < L.groups ? group_rows<T>(d.rows, seq, token, head, d.row_stride_seq, d.row_stride_token, d.row_stride_head) : nullptr;
-                    scale[u] = 0.0f;
-                    if (v[u] && token < tokens)
-                    {
-                        place    = group_place(L, seq, token, head);
-                        scale[u] = __uint_as_float(0x7fffffffu);
-                        if (place < 0 && at.l == 0 && d.status)
-                            *d.status = 1;
-                    }
-                    given[u] = place >= 0;
-                    codes[u] = static_cast<const uint8_t*>(d.codes) + place * d.dim;
-                    if (given[u])
-                    {
-                        scale[u] = d.scales[place];
-                        if constexpr (NC > 0)
-                        {
-#pragma unroll
-                            for (int j = 0; j < NC; ++j)
-                                if (j * L.lanes + at.l < chunks)
-                                    q[u][j].load(codes[u] + (j * L.lanes + at.l) * V);
-                        }
-                    }
+                    place = group_place(L, seq, token, head);
+                    scale = __uint_as_float(0x7fffffffu);
+                    if (place < 0 && at.l == 0 && d.status)
+                        *d.status = 1;
                 }
-#pragma unroll
-                for (int u = 0; u < U; ++u)
+                const uint8_t* codes = static_cast<const uint8_t*>(d.codes) + place * d.dim;
+                if (place >= 0)
                 {
-                    if (!v[u])
-                        continue;
-                    const auto put = [&](code_words<V>& w, int i) {
-                        chunk<T, V> c;
-                        if (!given[u])
-                            c.fill(scale[u]);
-                        else if constexpr (V == 1)
-                            c.v = decode<CODE>(w.w[0], scale[u]);
-                        else
-                            decode_words<T, CODE, V>(c, w.w, scale[u]);
-                        c.store(v[u] + (int64_t)i * V);
-                    };
+                    scale = d.scales[place];
                     if constexpr (NC > 0)
                     {
 #pragma unroll
                         for (int j = 0; j < NC; ++j)
-                            if (j * L.lanes + at.l < chunks)
-                                put(q[u][j], j * L.lanes + at.l);
+                            if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                                q[j].load(codes + i, L.lanes, d.dim - i);
                     }
-                    else
-                        for (int i = at.l; i < chunks; i += L.lanes)
-                        {
-                            if (given[u])
-                                q[u][0].load(codes[u] + (int64_t)i * V);
-                            put(q[u][0], i);
-                        }
                 }
+                const auto put = [&](const code_words<V>& q, int i) {
+                    C c;
+                    if (place < 0)
+                        c.fill(scale);
+                    else
+                        decode_chunk<T, CODE, V>(c, q, scale);
+                    c.store(v + i, L.lanes, d.dim - i);
+                };
+                if constexpr (NC > 0)
+                {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+                        if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                            put(q[j], i);
+                }
+                else
+                    for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
+                    {
+                        if (place >= 0)
+                            q[0].load(codes + i, L.lanes, d.dim - i);
+                        put(q[0], i);
+                    }
             }
         }
 
@@ -735,45 +730,35 @@ namespace aeonb
                 throw std::invalid_argument("negative stride");
         }
 
-        template <typename T, int CODE, int V, int NC, int U>
+        template <typename T, int CODE, int V, int NC>
         void launch_lanes(cache_launch& L, bool write, cudaStream_t stream)
         {
-            const int chunks  = L.d.dim / V;
+            const int chunks  = (L.d.dim + chunk<T, V>::N - 1) / chunk<T, V>::N;
             L.lanes           = NC ? (chunks + NC - 1) / NC : 32;
             L.by_lanes        = fast_divisor(L.lanes);
             const int at_once = 32 / L.lanes;
             const int warps   = (int)std::min<int64_t>(8, ((int64_t)L.groups + at_once - 1) / at_once);
-            const int each    = warps * at_once * U;
+            const int each    = warps * at_once;
             const dim3 grid((unsigned)(((int64_t)L.groups + each - 1) / each), (unsigned)std::min(L.d.seqs, 65535));
             if (write)
-                cache_write_kernel<T, CODE, V, NC, U><<<grid, warps * 32, 0, stream>>>(L);
+                cache_write_kernel<T, CODE, V, NC><<<grid, warps * 32, 0, stream>>>(L);
             else
-                cache_read_kernel<T, CODE, V, NC, U><<<grid, warps * 32, 0, stream>>>(L);
+                cache_read_kernel<T, CODE, V, NC><<<grid, warps * 32, 0, stream>>>(L);
         }
 
         template <typename T, int CODE, int V>
         void launch_chunks(cache_launch& L, bool write, cudaStream_t stream)
         {
-            const int chunks = L.d.dim / V;
-            if constexpr (V == 1)
-            {
-                // single values: four or eight a lane, so that what a lane finds out about its group serves more than one
-                if (chunks <= 32 * 4)
-                    return launch_lanes<T, CODE, V, 4, 2>(L, write, stream);
-                if (chunks <= 32 * 8)
-                    return launch_lanes<T, CODE, V, 8, 1>(L, write, stream);
-            }
+            const int chunks = (L.d.dim + chunk<T, V>::N - 1) / chunk<T, V>::N;
+            // Two chunks a lane: what a lane finds out about its group serves both.  64 x 4096 x 8 groups of 128 bf16 to int8 with values, one
+            // chunk and two groups in turn / two chunks / four: 0.33 / 0.26 / 0.26 ms; e4m3 0.38 / 0.32 / 0.34; groups of 64 floats
+            // 0.24 / 0.19 / 0.22; read back 0.14 / 0.13 / 0.13.
+            if (chunks <= 32 * 2)
+                launch_lanes<T, CODE, V, 2>(L, write, stream);
+            else if (chunks <= 32 * 4)
+                launch_lanes<T, CODE, V, 4>(L, write, stream);
             else
-            {
-                // Two chunks a lane: what a lane finds out about its group serves both.  64 x 4096 x 8 groups of 128 bf16 to int8 with values,
-                // one chunk and two groups in turn / two chunks / four: 0.33 / 0.26 / 0.26 ms; e4m3 0.38 / 0.32 / 0.34; groups of 64 floats
-                // 0.24 / 0.19 / 0.22; read back 0.14 / 0.13 / 0.13.
-                if (chunks <= 32 * 2)
-                    return launch_lanes<T, CODE, V, 2, 1>(L, write, stream);
-                if (chunks <= 32 * 4)
-                    return launch_lanes<T, CODE, V, 4, 1>(L, write, stream);
-            }
-            launch_lanes<T, CODE, V, 0, 1>(L, write, stream);
+                launch_lanes<T, CODE, V, 0>(L, write, stream);
         }
 
         // bytes that every group's first value lies on
@@ -811,7 +796,7 @@ namespace aeonb
             {
             case 32: launch_chunks<T, CODE, 32 / sizeof(T)>(L, write, stream); break;
             case 16: launch_chunks<T, CODE, 16 / sizeof(T)>(L, write, stream); break;
-            default: launch_chunks<T, CODE, 1>(L, write, stream); break;
+            default: launch_chunks<T, CODE, APART>(L, write, stream); break;
             }
         }
 
