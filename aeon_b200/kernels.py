@@ -312,11 +312,11 @@ def _device_tensor(ctx, name, t, dtype, shape=None):
     """Data pointer of a tensor on the context's GPU, or None for None."""
     if t is None:
         return None
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise ValueError("%s must be a tensor on cuda:%d" % (name, ctx.device))
     if t.dtype != dtype:
         raise ValueError("%s must have the type %s, not %s" % (name, dtype, t.dtype))
-    if shape is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+    if shape is not None and (t.shape != shape or not t.is_contiguous()):
         raise ValueError("%s must be contiguous with the shape %s, not %s" % (name, tuple(shape), tuple(t.shape)))
     return t.data_ptr()
 
@@ -342,6 +342,8 @@ class FeatureCache:
         _device_tensor(ctx, "scales", scales, torch.float32, codes.shape[:3])
         self.ctx, self.codes, self.scales = ctx, codes, scales
         self.pages, self.page_tokens, self.heads, self.dim = codes.shape
+        self._cache = (codes.data_ptr(), scales.data_ptr(), self.pages, self.page_tokens, self.heads, self.dim,
+                       L.CODE_INT8 if codes.dtype == torch.int8 else L.CODE_E4M3)
 
     @classmethod
     def allocate(cls, ctx, pages, page_tokens, heads, dim, code="int8"):
@@ -352,22 +354,22 @@ class FeatureCache:
         return cls(ctx, codes if code == "int8" else codes.view(torch.float8_e4m3fn),
                    torch.zeros((pages, page_tokens, heads), dtype=torch.float32, device=dev))
 
-    def _desc(self, seqs, tokens, table, start, length, status):
+    def _desc(self, name, rows, table, start, length, status, values=None):
+        """The descriptor of a call; rows and values are (seqs, tokens, heads, dim)."""
         ctx = self.ctx
-        d = L.CacheDesc()
-        d.codes, d.scales = self.codes.data_ptr(), self.scales.data_ptr()
-        d.pages, d.page_tokens, d.heads, d.dim = self.pages, self.page_tokens, self.heads, self.dim
-        d.code = L.CODE_INT8 if self.codes.dtype == torch.int8 else L.CODE_E4M3
+        seqs, tokens = rows.shape[0], rows.shape[1]
         if table.dim() != 2 or table.shape[0] != seqs or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError("table must be (%d, n) with the pages of a sequence side by side" % seqs)
-        d.table, d.table_stride, d.table_pages = _device_tensor(ctx, "table", table, torch.int32), table.stride(0), table.shape[1]
-        d.seqs, d.tokens = seqs, tokens
-        d.start = _device_tensor(ctx, "start", start, torch.int32, (seqs,))
-        d.length = _device_tensor(ctx, "length", length, torch.int32, (seqs,))
         if status is not None and status.numel() < 1:
             raise ValueError("status must hold a word")
-        d.status = _device_tensor(ctx, "status", status, torch.int32)
-        return d
+        by_seq, by_token, by_head, _ = rows.stride()
+        v_seq, v_token, v_head, _ = values.stride() if values is not None else (0, 0, 0, 0)
+        each = (seqs,)
+        return L.CacheDesc(
+            *self._cache, _device_tensor(ctx, "table", table, torch.int32), table.stride(0), table.shape[1], seqs, tokens,
+            _float_type(name, rows), _device_tensor(ctx, "start", start, torch.int32, each),
+            _device_tensor(ctx, "length", length, torch.int32, each), _device_tensor(ctx, name, rows, rows.dtype), by_seq, by_token, by_head,
+            _device_tensor(ctx, "values", values, rows.dtype), v_seq, v_token, v_head, _device_tensor(ctx, "status", status, torch.int32))
 
     def _rows(self, name, t):
         """The tensor as (seqs, tokens, heads, dim)."""
@@ -382,63 +384,66 @@ class FeatureCache:
         """Writes `rows` into the cache; with `values` (a tensor like rows, or rows itself) also the values that the codes stand
         for.  Rows of `values` behind a sequence's length are left as they are."""
         rows = self._rows("rows", rows)
-        d = self._desc(rows.shape[0], rows.shape[1], table, start, length, status)
-        d.dtype, d.rows = _float_type("rows", rows), _device_tensor(self.ctx, "rows", rows, rows.dtype)
-        d.row_stride_seq, d.row_stride_token, d.row_stride_head = rows.stride()[:3]
         if values is not None:
             values = self._rows("values", values)
             if values.shape != rows.shape:
                 raise ValueError("values must have the shape of rows")
-            d.values = _device_tensor(self.ctx, "values", values, rows.dtype)
-            d.value_stride_seq, d.value_stride_token, d.value_stride_head = values.stride()[:3]
-        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_write, d)
+        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_write, self._desc("rows", rows, table, start, length, status, values))
 
     def read(self, table, tokens, start=None, length=None, out=None, dtype=torch.float32, status=None):
         """The values of `tokens` tokens of each sequence, (seqs, tokens, heads, dim); zeros behind a sequence's length."""
         if out is None:
-            out = torch.empty((table.shape[0], tokens, self.heads, self.dim), dtype=dtype, device=self.codes.device)
+            out = self.codes.new_empty((table.shape[0], tokens, self.heads, self.dim), dtype=dtype)
         rows = self._rows("out", out)
         if rows.shape[0] != table.shape[0] or rows.shape[1] != tokens:
             raise ValueError("out must hold %d tokens of %d sequences" % (tokens, table.shape[0]))
-        d = self._desc(rows.shape[0], tokens, table, start, length, status)
-        d.dtype, d.rows = _float_type("out", rows), _device_tensor(self.ctx, "out", rows, rows.dtype)
-        d.row_stride_seq, d.row_stride_token, d.row_stride_head = rows.stride()[:3]
-        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_read, d)
+        _on_current_stream(self.ctx, self.ctx.lib.aeonb_cache_read, self._desc("out", rows, table, start, length, status))
         return out
 
 
-def _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad):
+def _distill_rows(name, t):
+    """The tensor as rows at one stride, their values side by side."""
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, t.shape[-1])
+        except RuntimeError:
+            raise ValueError("%s must have rows at one stride" % name) from None
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("the values of a row of %s must lie side by side" % name)
+    return t
+
+
+def _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, loss=None, lse=None, grad=None):
+    """The descriptor of a call (loss and lse as addresses), and the tensors that it stands on."""
     if logits.dim() < 2:
         raise ValueError("logits must be (..., vocab) with at least two dimensions")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     if ids.shape[:-1] != lead or ids.shape != teacher.shape:
         raise ValueError("ids and teacher must be (..., k) with the leading dimensions of logits")
-
-    def rows(name, t):
-        try:
-            t = t if t.dim() == 2 else t.view(-1, t.shape[-1])
-        except RuntimeError:
-            raise ValueError("%s must have rows at one stride" % name) from None
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError("the values of a row of %s must lie side by side" % name)
-        return t
-
-    d = L.DistillDesc()
-    d.dtype, d.logits = _float_type("logits", logits), _device_tensor(ctx, "logits", logits, logits.dtype)
-    n = logits.numel() // max(vocab, 1)
-    x = rows("logits", logits) if n else logits
-    d.logits_stride, d.rows, d.vocab, d.k = x.stride(0), n, vocab, ids.shape[-1]
+    x = _distill_rows("logits", logits) if logits.numel() else logits
     ids, teacher = ids.contiguous(), teacher.contiguous()
-    d.ids, d.teacher = _device_tensor(ctx, "ids", ids, torch.int32), _device_tensor(ctx, "teacher", teacher, torch.float32)
-    d.entry_stride, d.temperature = d.k, temperature
-    d.weights = _device_tensor(ctx, "weights", weights, torch.float32, lead)
-    d.upstream, d.grad_scale = _device_tensor(ctx, "upstream", upstream, torch.float32, lead), grad_scale
+    grad_at, grad_stride = None, 0
     if grad is not None:
         if grad.shape != logits.shape:
             raise ValueError("grad must have the shape of logits")
-        d.grad = _device_tensor(ctx, "grad", grad, logits.dtype)
-        d.grad_stride = (rows("grad", grad) if n else grad).stride(0)
-    return d, (ids, teacher)
+        grad_at = _device_tensor(ctx, "grad", grad, logits.dtype)
+        grad_stride = (_distill_rows("grad", grad) if grad.numel() else grad).stride(0)
+    k = ids.shape[-1]
+    return L.DistillDesc(
+        _device_tensor(ctx, "logits", logits, logits.dtype), x.stride(0), lead.numel(), vocab, _float_type("logits", logits),
+        _device_tensor(ctx, "ids", ids, torch.int32), _device_tensor(ctx, "teacher", teacher, torch.float32), k, k, temperature,
+        _device_tensor(ctx, "weights", weights, torch.float32, lead), loss, lse, grad_at, grad_stride,
+        _device_tensor(ctx, "upstream", upstream, torch.float32, lead), grad_scale), (ids, teacher)
+
+
+def _distill_grad_like(logits):
+    """A tensor for the gradient whose rows lie as those of the logits do, which is written fastest."""
+    if logits.is_contiguous() or logits.dim() < 2 or not logits.numel():
+        return torch.empty_like(logits)
+    x = _distill_rows("logits", logits)
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:  # a broadcast input
+        return logits.new_empty(logits.shape)
+    return torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype, device=logits.device)
 
 
 def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, want_grad=True, grad=None):
@@ -446,22 +451,26 @@ def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstr
     grad_scale * sum(upstream * loss) with respect to the logits, in one pass over them (aeonb_distill_loss).
 
     logits: (..., vocab) float32, float16 or bfloat16; ids (int32, -1 = no entry) and teacher (float32): (..., k), as the
-    "top_logits" etl type delivers them; weights, upstream: (...) float32.  Returns (loss, lse, grad); grad is None without
-    want_grad, and may be given (a tensor like logits, or logits itself).  A training step goes on with logits.backward(grad)."""
-    if want_grad and grad is None:
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad if want_grad else None)
-    both = torch.empty((2,) + tuple(logits.shape[:-1]), dtype=torch.float32, device=logits.device)
-    d.loss, d.lse = both.data_ptr(), both.data_ptr() + 4 * d.rows
+    "top_logits" etl type delivers them; weights, upstream: (...) float32.  Returns (loss, lse, grad); grad has the strides of the
+    logits, is None without want_grad, and may be given (a tensor like logits, or logits itself).  A training step goes on with
+    logits.backward(grad)."""
+    if not want_grad:
+        grad = None
+    elif grad is None:
+        grad = _distill_grad_like(logits)
+    both = logits.new_empty((2,) + logits.shape[:-1], dtype=torch.float32)
+    at = both.data_ptr()
+    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, at, at + 2 * both.numel(), grad)
     _on_current_stream(ctx, ctx.lib.aeonb_distill_loss, d)
-    return both[0], both[1], grad if want_grad else None
+    loss, lse = both.unbind(0)
+    return loss, lse, grad
 
 
 def distill_grad(ctx, logits, ids, teacher, lse, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, grad=None):
     """The gradient alone, from the lse that distill_loss returned for the same logits and temperature (aeonb_distill_grad)."""
     if grad is None:
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale, grad)
-    d.lse = _device_tensor(ctx, "lse", lse, torch.float32, logits.shape[:-1])
+        grad = _distill_grad_like(logits)
+    d, keep = _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, grad_scale,
+                            lse=_device_tensor(ctx, "lse", lse, torch.float32, logits.shape[:-1]), grad=grad)
     _on_current_stream(ctx, ctx.lib.aeonb_distill_grad, d)
     return grad
