@@ -435,6 +435,196 @@ namespace aeonb
             return make_float2(top, pow2(__fmul_rn(-__fmaf_rn(lse, L.d.temperature, -top), L.c)));
         }
 
+        // Rows of up to 128 values or 256 vectors with up to 32 entries: G lanes each, 32 / G rows to a warp, NV vectors a lane (VECTOR) or
+        // values.  Every lane takes part in every step, whatever its row.
+        struct few_entries
+        {
+            int   id[32];
+            float p[32], t[32], s[32];
+        };
+        template <int G, typename V, typename Op>
+        __device__ __forceinline__ V group_reduce(V v, Op op)
+        {
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1)
+                v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+            return v;
+        }
+
+        template <typename T, int MODE, int G, int NV, bool VECTOR>
+        __global__ void __launch_bounds__(256, 4) distill_few_kernel(const distill_launch L)
+        {
+            constexpr int N = piece<T>::N;
+            __shared__ few_entries    all[256 / G];
+            const aeonb_distill_desc& d   = L.d;
+            const int                 l   = threadIdx.x & (G - 1);
+            const int64_t             row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+            const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
+            few_entries&              e    = all[threadIdx.x / G];
+            const bool                real = row < d.rows;
+            const T*                  s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
+            const cut<T>              c(s, d.vocab);
+            const float               w   = !real ? 0.0f : d.weights ? d.weights[row] : 1.0f; // (its row is read without waiting for it)
+            piece<T>                  x[VECTOR ? NV : 1];
+            float                     one[VECTOR ? 2 : NV]; // single values; of a row in vectors, one before them and one behind
+            const auto at_one = [&](int j) { return !VECTOR ? (j * G + l < d.vocab ? j * G + l : -1)
+                                                  : j == 0  ? (l < c.head ? l : -1)
+                                                            : (l < c.tail ? c.head + c.n * N + l : -1); };
+            constexpr int ONES = VECTOR ? 2 : NV;
+#pragma unroll
+            for (int j = 0; j < ONES; ++j)
+                one[j] = real && at_one(j) >= 0 ? to_float(s[at_one(j)]) : -inf;
+            if constexpr (VECTOR)
+            {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (real && j * G + l < c.n)
+                        x[j].load(s + c.head + (j * G + l) * N);
+                    else
+                        x[j].clear();
+            }
+            float up = 1.0f, lse = 0.0f;
+            if (real && MODE != LOSS && d.upstream)
+                up = d.upstream[row];
+            if (real && MODE == GRAD)
+                lse = d.lse[row];
+            // the largest entry and the largest value, then the two sums, then the gradient; the loss last
+            float tmax = -inf, m = -inf;
+            int   odd  = 0;
+            for (int k = l; k < d.k; k += G)
+            {
+                int   id = -1;
+                float t  = -inf;
+                if (real)
+                    odd |= read_entry(d, row, k, id, t);
+                e.id[k] = id;
+                e.t[k]  = t;
+                e.s[k]  = id >= 0 && id < d.vocab ? to_float(s[id]) : 0.0f;
+                tmax    = fmaxf(tmax, t);
+            }
+            if (MODE != GRAD)
+            {
+#pragma unroll
+                for (int j = 0; j < ONES; ++j)
+                    m = fmaxf(m, one[j]);
+                if constexpr (VECTOR)
+                {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        m = x[j].largest(m);
+                }
+            }
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1)
+            {
+                const float a = __shfl_xor_sync(0xffffffffu, tmax, o), b = MODE != GRAD ? __shfl_xor_sync(0xffffffffu, m, o) : 0.0f;
+                odd |= __shfl_xor_sync(0xffffffffu, odd, o);
+                tmax = fmaxf(tmax, a);
+                m    = fmaxf(m, b);
+            }
+            const bool found = w != 0.0f && (odd || tmax != -inf);
+            bool       bad   = odd || !(tmax < inf);
+            float      esum = 0.0f, sum = 0.0f, top = m;
+            for (int k = l; k < d.k; k += G)
+            {
+                const float t = __fmul_rn(__fsub_rn(e.t[k], tmax), L.c);
+                const float p = e.id[k] >= 0 ? pow2(t) : 0.0f;
+                e.t[k]        = t;
+                e.p[k]        = p;
+                esum          = __fadd_rn(esum, p);
+            }
+            if (MODE != GRAD)
+            {
+                float2 z = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < ONES; ++j)
+                    z.x = __fadd_rn(z.x, pow2(__fmul_rn(__fsub_rn(one[j], top), L.c)));
+                if constexpr (VECTOR)
+                {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        z = x[j].sum(z, top, L.c);
+                }
+                sum = __fadd_rn(z.x, z.y);
+            }
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1)
+            {
+                const float a = __shfl_xor_sync(0xffffffffu, esum, o), b = MODE != GRAD ? __shfl_xor_sync(0xffffffffu, sum, o) : 0.0f;
+                esum = __fadd_rn(esum, a);
+                sum  = __fadd_rn(sum, b);
+            }
+            float fq, f = __fmul_rn(__fmul_rn(w, L.factor), up);
+            if (MODE != GRAD)
+            {
+                bad |= !(fabsf(top) < inf) || sum != sum;
+                fq = __fdiv_rn(f, sum);
+            }
+            else
+            {
+                const float2 at = against_lse(L, lse);
+                bad |= !(fabsf(lse) < inf);
+                top = at.x;
+                fq  = __fmul_rn(f, at.y);
+            }
+            if (bad)
+                fq = nan;
+            const float share = __fdiv_rn(1.0f, esum);
+            T*          grad  = static_cast<T*>(d.grad) + row * d.grad_stride;
+            if (MODE != LOSS && real)
+            {
+#pragma unroll
+                for (int j = 0; j < ONES; ++j)
+                    if (at_one(j) >= 0)
+                        grad[at_one(j)] = from_float<T>(found ? __fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one[j], top), L.c))) : 0.0f);
+                if constexpr (VECTOR)
+                {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (j * G + l < c.n)
+                            store_piece(grad + c.head + (j * G + l) * N, found ? x[j].gradient(top, L.c, fq) : make_uint4(0, 0, 0, 0), L.together);
+                }
+            }
+            const float zsum2 = log2f(sum), esum2 = log2f(esum);
+            float       term  = 0.0f; // p (log p - s / T + lse), to the base 2
+            for (int k = l; k < d.k; k += G)
+            {
+                const float p = __fmul_rn(e.p[k], share);
+                e.p[k]        = p;
+                if (MODE != GRAD && p > 0.0f)
+                    term = __fadd_rn(term, __fmul_rn(p, __fadd_rn(__fsub_rn(e.t[k], esum2),
+                                                                  __fadd_rn(zsum2, __fmul_rn(__fsub_rn(top, e.s[k]), L.c)))));
+            }
+            if (MODE != GRAD)
+            {
+                term = group_reduce<G>(term, add());
+                if (real && l == 0)
+                {
+                    const float loss  = __fmul_rn(__fmul_rn(w, L.tt), __fmul_rn(term, LN2));
+                    const float whole = __fadd_rn(__fdiv_rn(top, d.temperature), __fmul_rn(zsum2, LN2));
+                    write_loss(d, row, !found ? 0.0f : bad ? nan : loss, !found ? 0.0f : bad ? nan : whole);
+                }
+            }
+            if (MODE == LOSS)
+                return;
+            __syncwarp();
+            // (eight lanes have up to four entries each, and look through them all; those of a whole warp at most one)
+            bool twice = true;
+            if (G == 32)
+                twice = repeats(e.id, nullptr, d.k);
+            if (found && !bad)
+                for (int k = l; k < d.k; k += G)
+                {
+                    const int id = e.id[k];
+                    if (id < 0)
+                        continue;
+                    if (twice)
+                        entry_gradient(L, e.id, e.p, grad, k, id, e.s[k], top, f, fq);
+                    else
+                        grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(e.s[k], top), L.c))), __fmul_rn(f, e.p[k])));
+                }
+        }
+
         // Rows of up to 128 values (a value per lane and step) or 256 vectors: a warp each.
         template <typename T, int MODE, int NT, int NV, bool VECTOR>
         __global__ void __launch_bounds__(NT) distill_warp_kernel(const distill_launch L)
@@ -554,10 +744,19 @@ namespace aeonb
                         grad[j * 32 + lane] = from_float<T>(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(one[j], top), L.c))));
             }
             __syncwarp();
-            if (!bad)
-                for (int k = lane; k < d.k; k += 32)
-                    if (e.id[k] >= 0)
-                        entry_gradient(L, e.id, e.p, grad, k, e.id[k], e.s[k], top, f, fq);
+            if (bad)
+                return;
+            const bool twice = d.k > 32 || repeats(e.id, nullptr, d.k);
+            for (int k = lane; k < d.k; k += 32)
+            {
+                const int id = e.id[k];
+                if (id < 0)
+                    continue;
+                if (twice)
+                    entry_gradient(L, e.id, e.p, grad, k, id, e.s[k], top, f, fq);
+                else
+                    grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(e.s[k], top), L.c))), __fmul_rn(f, e.p[k])));
+            }
         }
 
         // ---- named barriers of a block: those who wait, and those who only say that they have come
@@ -1040,6 +1239,14 @@ namespace aeonb
             return cudaGetLastError();
         }
 
+        template <typename T, int MODE, int G, int NV, bool VECTOR>
+        cudaError_t launch_few(const distill_launch& L, cudaStream_t stream)
+        {
+            constexpr int ROWS = 256 / G;
+            distill_few_kernel<T, MODE, G, NV, VECTOR><<<(unsigned)((L.d.rows + ROWS - 1) / ROWS), 256, 0, stream>>>(L);
+            return cudaGetLastError();
+        }
+
         template <typename T, int MODE, int NT>
         cudaError_t launch_blocks(const distill_launch& L, cudaStream_t stream)
         {
@@ -1102,18 +1309,25 @@ namespace aeonb
         cudaError_t launch_mode(distill_launch& L, cudaStream_t stream)
         {
             const int64_t vocab = L.d.vocab, vectors = vocab * (int64_t)sizeof(T) / 16; // whole ones, at most
-            if (vocab <= 32)
-                return launch_warps<T, MODE, 256, 1, false>(L, stream);
-            if (vocab <= 64)
-                return launch_warps<T, MODE, 256, 2, false>(L, stream);
+            if (L.d.k <= 32 && (vocab <= 128 || vectors <= 32 * 8))
+            {
+                // lanes of a row: LATER
+                if (vocab <= 32)
+                    return launch_few<T, MODE, 8, 4, false>(L, stream);
+                if (vocab <= 64)
+                    return launch_few<T, MODE, 8, 8, false>(L, stream);
+                if (vocab <= 128)
+                    return launch_few<T, MODE, 8, 16, false>(L, stream);
+                if (vectors <= 8 * 4)
+                    return launch_few<T, MODE, 8, 4, true>(L, stream);
+                if (vectors <= 8 * 8)
+                    return launch_few<T, MODE, 8, 8, true>(L, stream);
+                if (vectors <= 16 * 8)
+                    return launch_few<T, MODE, 16, 8, true>(L, stream);
+                return launch_few<T, MODE, 32, 8, true>(L, stream);
+            }
             if (vocab <= 128)
                 return launch_warps<T, MODE, 256, 4, false>(L, stream);
-            if (vectors <= 32)
-                return launch_warps<T, MODE, 256, 1, true>(L, stream);
-            if (vectors <= 32 * 2)
-                return launch_warps<T, MODE, 256, 2, true>(L, stream);
-            if (vectors <= 32 * 4)
-                return launch_warps<T, MODE, 256, 4, true>(L, stream);
             if (vectors <= 32 * 8)
                 return launch_warps<T, MODE, 256, 8, true>(L, stream);
             // Threads of a block: 256 where there is a gradient and up to eight such blocks hold a row, else 512.  8192 rows of 131072 bf16
