@@ -763,6 +763,19 @@ namespace aeonb
         __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
         __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+        // Waits until at most n groups of copies are under way (n known when unrolled).
+        __device__ __forceinline__ void wait_copies(int n)
+        {
+            if (n == 0)
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            else if (n == 1)
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else if (n == 2)
+                asm volatile("cp.async.wait_group 2;" ::: "memory");
+            else
+                asm volatile("cp.async.wait_group 3;" ::: "memory");
+        }
+
         // Longer rows: the blocks of a cluster (LOSS, LOSS_GRAD), or any number of blocks (GRAD).  A block keeps its part of a row, up to NV
         // vectors for each of NT threads, in shared memory, and goes from row to row: each thread copies its vectors of the next row into
         // the place of those that it has used for the last time, so that memory is never idle.  No other thread touches them.
@@ -772,9 +785,8 @@ namespace aeonb
         template <typename T, int MODE, int NT>
         __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : 5) distill_block_kernel(const distill_launch L)
         {
-            constexpr int NV = BLOCK_VECTORS, CHUNK = 2, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
+            constexpr int NV = BLOCK_VECTORS, CHUNK = NT == 256 ? 4 : 2, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
             constexpr int SUMS = 1, RESULT = 2, WRITTEN = 3; // barriers
-            static_assert(CHUNKS == 4, "waits for four copies");
             struct outcome // of a row's sums
             {
                 float top, fq; // the gradient at v is fq 2^((s[v] - top) c), less the entries' part
@@ -858,31 +870,32 @@ namespace aeonb
 #pragma unroll
                         for (int q = 0; q < CHUNKS; ++q)
                         {
-                            if (MODE == LOSS || q == 0)
-                                asm volatile("cp.async.wait_group 3;" ::: "memory");
-                            else if (q == 1)
-                                asm volatile("cp.async.wait_group 2;" ::: "memory");
-                            else if (q == 2)
-                                asm volatile("cp.async.wait_group 1;" ::: "memory");
-                            else
-                                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            wait_copies(MODE == LOSS ? CHUNKS - 1 : CHUNKS - 1 - q);
                             if (q * CHUNK * NT < have)
                             {
                                 piece<T> x[CHUNK];
-                                vector(x[0], q * CHUNK);
-                                if ((q * CHUNK + 1) * NT < have)
-                                    vector(x[1], q * CHUNK + 1);
-                                else
-                                    x[1].clear();
-                                const float higher = x[1].largest(x[0].largest(m));
-                                const float scale  = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
-                                m                  = higher;
-                                z                  = x[1].sum(x[0].sum(mul2(z, make_float2(scale, scale)), m, L.c), m, L.c);
+                                float    higher = m;
+#pragma unroll
+                                for (int i = 0; i < CHUNK; ++i)
+                                {
+                                    if ((q * CHUNK + i) * NT < have)
+                                        vector(x[i], q * CHUNK + i);
+                                    else
+                                        x[i].clear();
+                                    higher = x[i].largest(higher);
+                                }
+                                const float scale = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
+                                m                 = higher;
+                                z                 = mul2(z, make_float2(scale, scale));
+#pragma unroll
+                                for (int i = 0; i < CHUNK; ++i)
+                                    z = x[i].sum(z, m, L.c);
                             }
                             if (MODE == LOSS)
                             {
-                                fetch(s_then + next.at, coming, q * CHUNK);
-                                fetch(s_then + next.at, coming, q * CHUNK + 1);
+#pragma unroll
+                                for (int i = 0; i < CHUNK; ++i)
+                                    fetch(s_then + next.at, coming, q * CHUNK + i);
                                 commit();
                             }
                         }
@@ -912,7 +925,7 @@ namespace aeonb
                             for (int j = 0; j < NV; ++j)
                             {
                                 if (MODE == GRAD && j % CHUNK == 0)
-                                    asm volatile("cp.async.wait_group 3;" ::: "memory");
+                                    wait_copies(CHUNKS - 1);
                                 if (j * NT < mine.left)
                                 {
                                     piece<T> x;
@@ -1331,8 +1344,8 @@ namespace aeonb
             if (vectors <= 32 * 8)
                 return launch_warps<T, MODE, 256, 8, true>(L, stream);
             // Threads of a block: 256 where there is a gradient and up to eight such blocks hold a row, else 512.  8192 rows of 131072 bf16
-            // logits, 256 / 512: with gradient 0.88 / 0.91 ms, gradient alone 0.74 / 0.80, loss alone 0.51 / 0.47 (where nothing waits for
-            // the other blocks, fewer of them cost less).
+            // logits, 256 / 512: with gradient 0.86 / 0.91 ms, gradient alone 0.72 / 0.80, loss alone 0.51 / 0.47 (where nothing waits for
+            // the other blocks, fewer of them cost less; one is enough for 65536 rows of 16384: 0.42 ms with 256).
             const bool    narrow = MODE == GRAD || (MODE == LOSS_GRAD && vectors <= 8 * BLOCK_VECTORS * 256);
             const int64_t most   = BLOCK_VECTORS * (narrow ? 256 : 512);
             // Blocks of a row: as many as hold it, and more while they do not fill the SMs and have 4 KB each.
