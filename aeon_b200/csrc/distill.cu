@@ -304,13 +304,14 @@ namespace aeonb
             return false;
         }
 
-        // The entries of a row, in shared memory.
+        // The entries of a row, up to ROOM of them, in shared memory.
+        template <int ROOM>
         struct entries
         {
-            int   id[ENTRIES];    // -1: none
-            float p[ENTRIES];     // teacher's probability
-            float t[ENTRIES];     // (t - largest t) c
-            float s[ENTRIES];     // the student's logit at id
+            int   id[ROOM]; // -1: none
+            float p[ROOM];  // teacher's probability
+            float t[ROOM];  // (t - largest t) c
+            float s[ROOM];  // the student's logit at id
         };
 
         // An entry: its id (-1 where it does not count) and the teacher's logit; true where the row is NaN for it.
@@ -326,8 +327,8 @@ namespace aeonb
 
         // A warp reads a row's entries and forms their probabilities; returns the log2 of their sum.  found: whether there are any;
         // bad: an id outside the vocabulary, or teacher's logits without a finite largest one.
-        template <typename T>
-        __device__ __forceinline__ float read_entries(const distill_launch& L, int64_t row, const T* s, entries& e, bool& found, bool& bad)
+        template <typename T, int ROOM>
+        __device__ __forceinline__ float read_entries(const distill_launch& L, int64_t row, const T* s, entries<ROOM>& e, bool& found, bool& bad)
         {
             const aeonb_distill_desc& d    = L.d;
             const int                 lane = threadIdx.x & 31;
@@ -364,7 +365,8 @@ namespace aeonb
         }
 
         // The loss of a row, by the warp that has read its entries.
-        __device__ __forceinline__ float entries_loss(const distill_launch& L, const entries& e, float esum2, float top, float zsum2, float w)
+        template <int ROOM>
+        __device__ __forceinline__ float entries_loss(const distill_launch& L, const entries<ROOM>& e, float esum2, float top, float zsum2, float w)
         {
             float term = 0.0f; // p (log p - s / T + lse), to the base 2
             for (int k = threadIdx.x & 31; k < L.d.k; k += 32)
@@ -391,7 +393,9 @@ namespace aeonb
                 grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(s, top), L.c))), __fmul_rn(f, all)));
         }
 
-        // Whether an id occurs more than once among a row's entries: a warp enters them into a table of twice as many places.
+        // Whether an id occurs more than once among a row's entries: a warp enters them into a table of at least twice as many places.
+        constexpr int PLACES = 512;
+        static_assert(PLACES == 1 << 9 && PLACES >= 2 * ENTRIES, "the hash below has nine bits");
         __device__ __forceinline__ bool repeats(const int* ids, int* table, int k)
         {
             const int lane = threadIdx.x & 31;
@@ -401,14 +405,14 @@ namespace aeonb
                 const unsigned same = __match_any_sync(0xffffffffu, id); // (all lanes take part)
                 return __any_sync(0xffffffffu, id >= 0 && __popc(same) > 1);
             }
-            for (int i = lane; i < 2 * ENTRIES; i += 32)
+            for (int i = lane; i < PLACES; i += 32)
                 table[i] = -1;
             __syncwarp();
             bool twice = false;
             for (int i = lane; i < k; i += 32)
             {
                 const int id = ids[i];
-                for (uint32_t at = (uint32_t)id * 2654435761u >> 23; id >= 0; at = (at + 1) & (2 * ENTRIES - 1))
+                for (uint32_t at = (uint32_t)id * 2654435761u >> (32 - 9); id >= 0; at = (at + 1) & (PLACES - 1))
                 {
                     const int there = atomicCAS(&table[at], -1, id); // (which of two equal ones enters does not matter)
                     twice |= there == id;
@@ -416,7 +420,6 @@ namespace aeonb
                         break;
                 }
             }
-            static_assert(2 * ENTRIES == 1 << (32 - 23), "the hash has as many values as the table places");
             return __any_sync(0xffffffffu, twice);
         }
 
@@ -636,7 +639,7 @@ namespace aeonb
             const float               inf = __uint_as_float(0x7f800000u), nan = __uint_as_float(0x7fffffffu);
             if (row >= d.rows)
                 return;
-            entries& e    = reinterpret_cast<entries*>(dynamic)[threadIdx.x / 32];
+            auto&    e    = reinterpret_cast<entries<ENTRIES>*>(dynamic)[threadIdx.x / 32];
             const T* s    = static_cast<const T*>(d.logits) + row * d.logits_stride;
             T*       grad = MODE == LOSS ? nullptr : static_cast<T*>(d.grad) + row * d.grad_stride;
 
@@ -782,10 +785,10 @@ namespace aeonb
         // The last warp has no vectors.  It reads the entries of the next row while the others work on this one, puts the warps' sums
         // (and the other blocks') together, hands out what the gradient needs, and writes the entries' own part when the rest is there.
         // So the others wait once in a row, from their last exponential to the first store.
-        template <typename T, int MODE, int NT>
-        __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : 5) distill_block_kernel(const distill_launch L)
+        template <typename T, int MODE, int NT, int ROOM>
+        __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : NT == 256 ? 5 : NT == 128 ? 9 : 15) distill_block_kernel(const distill_launch L)
         {
-            constexpr int NV = BLOCK_VECTORS, CHUNK = NT == 256 ? 4 : 2, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
+            constexpr int NV = BLOCK_VECTORS, CHUNK = NT == 512 ? 2 : 4, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
             constexpr int SUMS = 1, RESULT = 2, WRITTEN = 3; // barriers
             struct outcome // of a row's sums
             {
@@ -795,9 +798,9 @@ namespace aeonb
             };
             extern __shared__ __align__(16) unsigned char dynamic[]; // NV x NT vectors
             __shared__ float2   part[WARPS], theirs[2][16];
-            __shared__ entries  of_row[2]; // of this row and of the next one
+            __shared__ entries<ROOM> of_row[2]; // of this row and of the next one
             __shared__ outcome  result;
-            __shared__ int      table[2 * ENTRIES];
+            __shared__ int      table[PLACES];
             __shared__ uint64_t arrived[2];
             const aeonb_distill_desc& d    = L.d;
             const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -975,7 +978,7 @@ namespace aeonb
                     float esum2;
                     bool  found, bad;
                 };
-                const auto prepare = [&](int64_t r, float w, const T* s, entries& e) {
+                const auto prepare = [&](int64_t r, float w, const T* s, entries<ROOM>& e) {
                     facts a{w, 1.0f, 0.0f, 0.0f, false, false};
                     if (w == 0.0f)
                         return a;
@@ -1032,7 +1035,7 @@ namespace aeonb
                 for (int turn = 0; row < d.rows; row += step, ++turn)
                 {
                     const int      set = turn & 1;
-                    const entries& e   = of_row[set];
+                    const auto&    e   = of_row[set];
                     const float    w_after = weight(row + 2 * step);
                     float          top = 0.0f, z = 1.0f;
                     bool           bad = now.bad;
@@ -1137,7 +1140,7 @@ namespace aeonb
         __global__ void __launch_bounds__(THREADS) distill_kernel(const distill_launch L)
         {
             __shared__ float          shared[THREADS / 32];
-            __shared__ entries        e;
+            __shared__ entries<ENTRIES> e;
             __shared__ float          esum2_;
             __shared__ int            flags;
             const aeonb_distill_desc& d    = L.d;
@@ -1248,7 +1251,7 @@ namespace aeonb
         {
             constexpr int ROWS   = NT / 32;
             const int64_t blocks = (L.d.rows + ROWS - 1) / ROWS;
-            distill_warp_kernel<T, MODE, NT, NV, VECTOR><<<(unsigned)blocks, NT, sizeof(entries) * ROWS, stream>>>(L);
+            distill_warp_kernel<T, MODE, NT, NV, VECTOR><<<(unsigned)blocks, NT, sizeof(entries<ENTRIES>) * ROWS, stream>>>(L);
             return cudaGetLastError();
         }
 
@@ -1260,10 +1263,10 @@ namespace aeonb
             return cudaGetLastError();
         }
 
-        template <typename T, int MODE, int NT>
+        template <typename T, int MODE, int NT, int ROOM>
         cudaError_t launch_blocks(const distill_launch& L, cudaStream_t stream)
         {
-            auto                kernel = distill_block_kernel<T, MODE, NT>;
+            auto                kernel = distill_block_kernel<T, MODE, NT, ROOM>;
             cudaLaunchConfig_t  cfg    = {};
             cudaLaunchAttribute attr   = {};
             cfg.blockDim         = dim3(NT + 32);
@@ -1363,8 +1366,16 @@ namespace aeonb
             L.vectors = (int)(((vectors + blocks - 1) / blocks + 7) / 8 * 8); // whole lines of 128 bytes
             if constexpr (MODE != GRAD)
                 if (L.vectors > BLOCK_VECTORS * 256)
-                    return launch_blocks<T, MODE, 512>(L, stream);
-            return launch_blocks<T, MODE, 256>(L, stream);
+                    return launch_blocks<T, MODE, 512, ENTRIES>(L, stream);
+            if (L.d.k > 64)
+                return launch_blocks<T, MODE, 256, ENTRIES>(L, stream);
+            // shorter parts: fewer threads and more blocks to an SM, unless all blocks have one to themselves
+            const bool alone = L.d.rows * blocks <= 148;
+            if (L.vectors <= BLOCK_VECTORS * 64 && !alone)
+                return launch_blocks<T, MODE, 64, 64>(L, stream);
+            if (L.vectors <= BLOCK_VECTORS * 128 && !alone)
+                return launch_blocks<T, MODE, 128, 64>(L, stream);
+            return launch_blocks<T, MODE, 256, 64>(L, stream);
         }
 
         template <typename T>
