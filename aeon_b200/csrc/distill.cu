@@ -393,17 +393,18 @@ namespace aeonb
                 grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(s, top), L.c))), __fmul_rn(f, all)));
         }
 
-        // Whether an id occurs more than once among a row's entries: a warp enters them into a table of at least twice as many places.
+        // Whether an id in [from, to) occurs more than once among a row's entries: a warp enters them into a table of at least twice as many
+        // places.
         constexpr int PLACES = 512;
         static_assert(PLACES == 1 << 9 && PLACES >= 2 * ENTRIES, "the hash below has nine bits");
-        __device__ __forceinline__ bool repeats(const int* ids, int* table, int k)
+        __device__ __forceinline__ bool repeats(const int* ids, int* table, int k, int from, int to)
         {
             const int lane = threadIdx.x & 31;
             if (k <= 32)
             {
                 const int      id   = lane < k ? ids[lane] : -1;
                 const unsigned same = __match_any_sync(0xffffffffu, id); // (all lanes take part)
-                return __any_sync(0xffffffffu, id >= 0 && __popc(same) > 1);
+                return __any_sync(0xffffffffu, id >= from && id < to && __popc(same) > 1);
             }
             for (int i = lane; i < PLACES; i += 32)
                 table[i] = -1;
@@ -412,7 +413,7 @@ namespace aeonb
             for (int i = lane; i < k; i += 32)
             {
                 const int id = ids[i];
-                for (uint32_t at = (uint32_t)id * 2654435761u >> (32 - 9); id >= 0; at = (at + 1) & (PLACES - 1))
+                for (uint32_t at = (uint32_t)id * 2654435761u >> (32 - 9); id >= from && id < to; at = (at + 1) & (PLACES - 1))
                 {
                     const int there = atomicCAS(&table[at], -1, id); // (which of two equal ones enters does not matter)
                     twice |= there == id;
@@ -614,7 +615,7 @@ namespace aeonb
             // (eight lanes have up to four entries each, and look through them all; those of a whole warp at most one)
             bool twice = true;
             if (G == 32)
-                twice = repeats(e.id, nullptr, d.k);
+                twice = repeats(e.id, nullptr, d.k, 0, d.vocab);
             if (found && !bad)
                 for (int k = l; k < d.k; k += G)
                 {
@@ -749,7 +750,7 @@ namespace aeonb
             __syncwarp();
             if (bad)
                 return;
-            const bool twice = d.k > 32 || repeats(e.id, nullptr, d.k);
+            const bool twice = d.k > 32 || repeats(e.id, nullptr, d.k, 0, d.vocab);
             for (int k = lane; k < d.k; k += 32)
             {
                 const int id = e.id[k];
@@ -1110,7 +1111,7 @@ namespace aeonb
                         const cut<T> c(s, d.vocab);
                         const int    begin = min(rank * L.vectors, c.n), end = min(begin + L.vectors, c.n);
                         const int    from = first ? 0 : c.head + begin * N, to = last ? d.vocab : c.head + end * N;
-                        const bool   twice = here.found && !bad && repeats(e.id, table, d.k);
+                        const bool   twice = here.found && !bad && repeats(e.id, table, d.k, from, to);
                         bar_sync(WRITTEN, ALL);
                         if (here.found && !bad)
                             for (int k = lane; k < d.k; k += 32)
@@ -1226,9 +1227,8 @@ namespace aeonb
                 throw std::invalid_argument("the logits need between 0 and 2^31-1 rows of between 1 and 2^30 values");
             if (d.k < 1 || d.k > ENTRIES)
                 throw std::invalid_argument("a row has between 1 and 256 entries");
-            if (!(d.temperature > 0.0f) || !std::isfinite(d.temperature) || !std::isfinite(1.4426950408889634 / d.temperature) ||
-                !std::isfinite(d.temperature * d.temperature))
-                throw std::invalid_argument("the temperature must be a positive number");
+            if (!(d.temperature >= 0x1p-40f && d.temperature <= 0x1p40f))
+                throw std::invalid_argument("the temperature must be a number between 2^-40 and 2^40");
             if (d.rows == 0)
                 return;
             if (!d.logits || !d.ids || !d.teacher)

@@ -750,6 +750,16 @@ namespace aeonb
         void launch_chunks(cache_launch& L, bool write, cudaStream_t stream)
         {
             const int chunks = (L.d.dim + chunk<T, V>::N - 1) / chunk<T, V>::N;
+            if (V == APART && chunks > 32 && chunks <= 32 * 3)
+            {
+                // as many chunks a lane as leave the fewest lanes without values (161 values: 14 lanes with three, two groups to a warp)
+                const auto idle = [&](int n) {
+                    const int lanes = (chunks + n - 1) / n;
+                    return lanes > 32 ? 1.0 : 1.0 - (double)(32 / lanes) * L.d.dim / (32.0 * 4 * n);
+                };
+                if (idle(3) < idle(2) && idle(3) <= idle(4))
+                    return launch_lanes<T, CODE, V, 3>(L, write, stream);
+            }
             // Two chunks a lane: what a lane finds out about its group serves both.  64 x 4096 x 8 groups of 128 bf16 to int8 with values, one
             // chunk and two groups in turn / two chunks / four: 0.33 / 0.26 / 0.26 ms; e4m3 0.38 / 0.32 / 0.34; groups of 64 floats
             // 0.24 / 0.19 / 0.22; read back 0.14 / 0.13 / 0.13.

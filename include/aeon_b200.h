@@ -341,7 +341,8 @@ int64_t aeonb_specgram_bytes(const aeonb_specgram_desc* descs, int n, const aeon
  *     and does not count in max|x|.  A group that holds a NaN or +infinity gets the scale NaN and reads back as NaN.
  *
  *     aeonb_cache_write puts tokens [start[s], start[s] + n) of each sequence, n = min(length[s], tokens), into their pages;
- *     with `values` it also writes the values the codes stand for (`values` may be `rows` itself with the same strides).
+ *     with `values` it also writes the values the codes stand for (`values` may be `rows` itself with the same strides, and must not
+ *     share memory with them otherwise).
  *     Rows of `values` behind the n-th are left as they are.  The pages of one call's sequences must differ (two tokens
  *     written to one place leave either's bytes there, or some of both).
  *     aeonb_cache_read writes the values of the same tokens to `rows`; rows behind the n-th are filled with zeros, as behind
@@ -404,7 +405,8 @@ int aeonb_cache_read(aeonb_ctx* ctx, const aeonb_cache_desc* desc);
  *     an id >= vocab, or whose largest logit is not finite, has loss, lse and gradient NaN.
  *
  *     aeonb_distill_loss writes loss and lse (either may be NULL) and, where grad is given, the gradient in the same pass.
- *     aeonb_distill_grad writes the gradient from the lse of an earlier call.  grad may be logits itself, with the same stride.
+ *     aeonb_distill_grad writes the gradient from the lse of an earlier call.  grad may be logits itself, with the same stride; otherwise
+ *     no output may share memory with an input.
  *     A gradient whose rows lie in their 16 bytes as the logits' rows
  *     do (any with the logits' stride and alignment) is written in whole vectors, another one value by value.
  *     Both run on the context's stream or the one given (cudaStreamLegacy for the default stream), make no allocation, copy
@@ -424,7 +426,7 @@ typedef struct aeonb_distill_desc
     const float* teacher;   /* device: rows x k */
     int64_t entry_stride;   /* elements between the rows of ids and of teacher */
     int32_t k;              /* 1..AEONB_DISTILL_MAX_ENTRIES */
-    float   temperature;    /* > 0 */
+    float   temperature;    /* 2^-40..2^40 */
     const float* weights;   /* device: one per row; NULL: 1 */
     float*  loss;           /* device: one per row */
     float*  lse;            /* device: one per row; read by aeonb_distill_grad */

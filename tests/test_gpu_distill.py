@@ -330,6 +330,58 @@ def test_two_captured_graphs(ctx, vocab):
             assert torch.equal(alone, K.distill_grad(ctx, logits, ids, teacher, want[1], 2.0))
 
 
+def test_a_first_call_inside_a_capture(ctx):
+    """Sizes and entries that no other test uses: what the library asks the driver for at their first call is allowed there."""
+    from aeon_b200 import kernels as K
+    rng = np.random.default_rng(20)
+    for vocab, k in ((9001, 70), (70003, 129)):
+        logits, ids, teacher = make(rng, 300, vocab, k, "f16")
+        logits = logits.contiguous()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = K.distill_loss(ctx, logits, ids, teacher, 2.0)
+        g.replay()
+        torch.cuda.synchronize()
+        again = K.distill_loss(ctx, logits, ids, teacher, 2.0)
+        assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+@pytest.mark.parametrize("k", [31, 33, 64, 65, 200])
+@pytest.mark.parametrize("vocab", [100, 700, 3000, 9000, 40000, 140000])
+def test_many_entries_with_repeats(ctx, k, vocab):
+    """Entry counts around those at which the kernels change, ids that occur often, all at one end of the row or spread."""
+    rng = np.random.default_rng(k * 7 + vocab)
+    logits, ids, teacher = make(rng, 4, vocab, k, "f32", 3)
+    ids[0] = ids[0] % 7 + vocab - 7
+    ids[1] = torch.arange(k, dtype=torch.int32) % vocab
+    ids[2, ::2] = ids[2, 0]
+    ids[2, 1::3] = -1
+    check(ctx, logits, ids, teacher, 1.5, [1.0, -0.5, 2.0, 1.0], [1.0, 2.0, 0.5, -1.0])
+
+
+def test_temperatures_at_the_ends(ctx):
+    """The coldest and the hottest temperature: all on the largest value, all alike."""
+    rng = np.random.default_rng(21)
+    for vocab in (50, 5000, 50000):
+        for t in (2.0 ** -40, 2.0 ** 40):
+            logits, ids, teacher = make(rng, 3, vocab, 5, "f32")
+            from aeon_b200 import kernels as K
+            loss, lse, grad = K.distill_loss(ctx, logits, ids, teacher, t)
+            assert lse.isfinite().all() and grad.isfinite().all()
+            top = logits.max(1).values.double()
+            if t < 1:  # q is 1 at the largest value and 0 elsewhere, p too
+                want = torch.zeros(3, vocab, dtype=torch.float64, device="cuda")
+                want.scatter_add_(1, logits.argmax(1, keepdim=True), torch.full((3, 1), t, dtype=torch.float64, device="cuda"))
+                want.scatter_add_(1, ids.gather(1, teacher.argmax(1, keepdim=True)).long(), torch.full((3, 1), -t, dtype=torch.float64, device="cuda"))
+                assert (grad.double() - want).abs().max().item() <= t * 2.0 ** -20
+                assert ((lse.double() * t - top).abs() <= top.abs() * 2.0 ** -22).all()
+            else:
+                want = torch.full((3, vocab), t / vocab, dtype=torch.float64, device="cuda")
+                want.scatter_add_(1, ids.long(), torch.full((3, 5), -t / 5, dtype=torch.float64, device="cuda"))
+                assert (grad.double() - want).abs().max().item() <= t * 2.0 ** -20
+
+
 def test_offsets_past_32_bits(ctx):
     """Rows so far apart that byte and element offsets pass 2^32."""
     from aeon_b200 import kernels as K

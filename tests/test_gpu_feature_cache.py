@@ -332,6 +332,52 @@ def test_pages_past_32_bits(ctx):
         del out, c
 
 
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_million_quotients(ctx, code, dtype):
+    """Codes of many groups of many sizes, in vectors and value by value: bit for bit those of the exact quotient."""
+    rng = np.random.default_rng(50)
+    for dim in (512, 77):
+        rows = features(rng, (2000, 1, 1, dim), dtype)
+        rows[::5] = (rows[::5] * 64 / rows[::5].abs().amax(-1, keepdim=True)).round()  # small whole numbers: many middles
+        c = cache(ctx, 2000, 1, 1, dim, code)
+        c.write(rows, torch.arange(2000, dtype=torch.int32, device="cuda")[:, None])
+        q, s = ocache.encode(rows.double().cpu().numpy(), code)
+        got = held(c)
+        assert np.array_equal(got[1][:, 0, 0], s[:, 0, 0])
+        assert np.array_equal(got[0][:, 0, 0], q[:, 0, 0])
+
+
+def test_more_sequences_than_a_grid_is_high(ctx):
+    rng = np.random.default_rng(51)
+    seqs = 70001
+    for dim, dtype in ((4, "f32"), (16, "bf16")):
+        rows = features(rng, (seqs, 1, 1, dim), dtype)
+        c = cache(ctx, seqs, 1, 1, dim, "int8")
+        table = torch.randperm(seqs, device="cuda").to(torch.int32)[:, None]
+        values = torch.empty_like(rows)
+        c.write(rows, table, values=values)
+        assert torch.equal(c.read(table, 1, dtype=TYPES[dtype]), values)
+        q, s = ocache.encode(rows.double().cpu().numpy(), "int8")
+        assert np.array_equal(held(c)[1][table[:, 0].cpu().numpy(), 0, 0], s[:, 0, 0])
+
+
+def test_positions_past_31_bits(ctx):
+    """Pages so long that a token's position passes 2^31."""
+    from aeon_b200 import kernels as K
+    rng = np.random.default_rng(52)
+    page = 2 ** 30
+    c = K.FeatureCache(ctx, torch.empty(3, page, 1, 1, dtype=torch.int8, device="cuda"), torch.empty(3, page, 1, device="cuda"))
+    table = torch.tensor([[1, 0, 2]], dtype=torch.int32, device="cuda")
+    rows = features(rng, (1, 6, 1, 1), "f32")
+    start = torch.tensor([2 ** 31 - 3], dtype=torch.int32, device="cuda")
+    values = torch.empty_like(rows)
+    c.write(rows, table, start=start, values=values)
+    assert torch.equal(c.read(table, 6, start=start), values)
+    q, s = ocache.encode(rows.double().cpu().numpy(), "int8")
+    assert np.array_equal(c.scales[0, page - 3:, 0].cpu().numpy(), s[0, :3, 0]) and np.array_equal(c.scales[2, :3, 0].cpu().numpy(), s[0, 3:, 0])
+
+
 def test_random_cases_round_trip(ctx):
     rng = np.random.default_rng(49)
     for _ in range(30):

@@ -84,7 +84,7 @@ BAD_DISTILL = [
     (dict(dtype=L.U8), "type of the rows"), (dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(vocab=0), "rows"), (dict(vocab=(1 << 30) + 1), "rows"),
     (dict(k=0), "entries"), (dict(k=257), "entries"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
-    (dict(temperature=float("inf")), "temperature"),
+    (dict(temperature=float("inf")), "temperature"), (dict(temperature=1e-13), "temperature"), (dict(temperature=2e12), "temperature"),
     (dict(logits=None), "NULL"), (dict(ids=None), "NULL"), (dict(teacher=None), "NULL"),
     (dict(logits=65537), "aligned"), (dict(grad=131073), "aligned"), (dict(ids=4098), "aligned"), (dict(teacher=8194), "aligned"),
     (dict(weights=2), "aligned"), (dict(upstream=1), "aligned"), (dict(loss=16386), "aligned"), (dict(lse=20482), "aligned"),
