@@ -178,8 +178,10 @@ namespace aeonb
             const float2 t = mul2(x, by.small);
             const float2 y = fma2_cut(fma2(t, by.scale, x), by.large, t);
             const float2 r = fma2(y, by.scale, x);
-            return make_float2(__uint_as_float(__float_as_uint(y.x) | (r.x != 0.0f ? 1u : 0u)),
-                               __uint_as_float(__float_as_uint(y.y) | (r.y != 0.0f ? 1u : 0u)));
+            uint32_t a, b; // all ones where something was cut
+            asm("set.ne.u32.f32 %0, %1, 0f00000000;" : "=r"(a) : "f"(r.x));
+            asm("set.ne.u32.f32 %0, %1, 0f00000000;" : "=r"(b) : "f"(r.y));
+            return make_float2(__uint_as_float(__float_as_uint(y.x) | (a & 1u)), __uint_as_float(__float_as_uint(y.y) | (b & 1u)));
         }
 
         // Codes of four finite values at once (in the order of the bytes); for int8 the values become the codes' numbers.
@@ -760,10 +762,12 @@ namespace aeonb
                 if (idle(3) < idle(2) && idle(3) <= idle(4))
                     return launch_lanes<T, CODE, V, 3>(L, write, stream);
             }
-            // Two chunks a lane: what a lane finds out about its group serves both.  64 x 4096 x 8 groups of 128 bf16 to int8 with values, one
-            // chunk and two groups in turn / two chunks / four: 0.33 / 0.26 / 0.26 ms; e4m3 0.38 / 0.32 / 0.34; groups of 64 floats
-            // 0.24 / 0.19 / 0.22; read back 0.14 / 0.13 / 0.13.
-            if (chunks <= 32 * 2)
+            // Four chunks a lane where that leaves a thousand lanes to an SM, else two: what a lane finds out about its group serves them all.
+            // 64 x 4096 x 8 groups of 128 bf16 with values, two / four: to e4m3 0.24 / 0.23 ms, to int8 0.24 / 0.22, read back
+            // 0.13 / 0.13; 2560 x 2000 groups of 40 floats to int8 0.37 / 0.35, read back 0.20 / 0.18; 256 x 200 of them, half there,
+            // 10.3 / 12.3 us.
+            const bool many = (int64_t)L.d.seqs * L.groups * chunks / 4 >= 148 * 1024;
+            if (chunks <= 32 * 2 && !(many && chunks >= 4 && V != APART))
                 launch_lanes<T, CODE, V, 2>(L, write, stream);
             else if (chunks <= 32 * 4)
                 launch_lanes<T, CODE, V, 4>(L, write, stream);
