@@ -445,13 +445,16 @@ def _distill_desc(ctx, logits, ids, teacher, temperature, weights, upstream, gra
 
 
 def _distill_grad_like(logits):
-    """A tensor for the gradient whose rows lie as those of the logits do, which is written fastest."""
-    if logits.is_contiguous() or logits.dim() < 2 or not logits.numel():
-        return torch.empty_like(logits)
+    """A tensor for the gradient whose rows lie in their 16 bytes as those of the logits do, which is written fastest."""
+    off = logits.data_ptr() % 16 // logits.element_size()  # of a view into the middle of a tensor
+    contiguous = logits.is_contiguous()
+    if contiguous and not off or logits.dim() < 2 or not logits.numel():
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
     x = _distill_rows("logits", logits)
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:  # a broadcast input
         return logits.new_empty(logits.shape)
-    return torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype, device=logits.device)
+    span = off + (x.shape[0] - 1) * x.stride(0) + x.shape[1]
+    return logits.new_empty(span).as_strided(logits.shape, logits.stride(), off)
 
 
 def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, want_grad=True, grad=None):

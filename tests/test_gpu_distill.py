@@ -243,6 +243,30 @@ def test_gradient_in_place(ctx, vocab, pad):
     assert torch.equal(b, alone)
 
 
+def test_gradients_lie_as_the_logits_do(ctx):
+    """Views into the middle of a tensor, padded and broadcast rows: the gradient has the logits' strides and place in 16 bytes where it
+    can, and the same values wherever it is written."""
+    from aeon_b200 import kernels as K
+    rng = np.random.default_rng(22)
+    for dtype in TYPES:
+        for vocab in (29, 501, 9001):
+            whole, ids, teacher = make(rng, 9, vocab, 5, dtype)
+            whole = whole.contiguous()
+            padded = torch.zeros(9, vocab + 7, dtype=TYPES[dtype], device="cuda")[:, 3:vocab + 3]
+            padded.copy_(whole)
+            for x, i, t in ((whole[1:], ids[1:], teacher[1:]), (whole[2:7], ids[2:7], teacher[2:7]), (padded, ids, teacher), (padded[4:], ids[4:], teacher[4:])):
+                loss, lse, grad = K.distill_loss(ctx, x, i, t, 2.0)
+                assert grad.shape == x.shape and grad.stride() == x.stride() and (grad.data_ptr() - x.data_ptr()) % 16 == 0
+                elsewhere = torch.empty(x.shape[0], vocab + 1, dtype=x.dtype, device="cuda")[:, 1:]
+                K.distill_loss(ctx, x, i, t, 2.0, grad=elsewhere)
+                assert torch.equal(elsewhere, grad)
+                assert torch.equal(K.distill_grad(ctx, x, i, t, lse, 2.0), K.distill_grad(ctx, x, i, t, lse, 2.0, grad=elsewhere))
+            same = K.distill_loss(ctx, whole[:1].expand(4, vocab), ids[:4], teacher[:4], 2.0)
+            assert same[2].is_contiguous()
+            one = [K.distill_loss(ctx, whole[:1], ids[j:j + 1], teacher[j:j + 1], 2.0) for j in range(4)]
+            assert torch.equal(same[0], torch.cat([o[0] for o in one])) and torch.equal(same[2], torch.cat([o[2] for o in one]))
+
+
 def test_what_lies_around_the_outputs_stays(ctx):
     from aeon_b200 import kernels as K
     rng = np.random.default_rng(14)
