@@ -6,8 +6,8 @@
 //
 // Measured on B200, 6.55 TB/s being what a copy reaches (events around a call, inputs not in L2): 64 x 4096 x 8 groups of 128 bf16 with
 // values to e4m3 0.23 ms (5.9 TB/s), to int8 0.22 (6.2), read back 0.13 (6.3); of 64 floats 0.20 (6.1) and 0.11 (6.3); 2560 x 2000 of
-// 40 floats 0.35 (5.4) and 0.18 (5.7); rows off 16 bytes less: 2560 x 200 of 161 floats 0.24 (3.2) and 0.13 (3.2), 5120 x 3330 of 13
-// 1.0 (2.1) and 0.51 (2.3), which wait for the issue of instructions.
+// 40 floats 0.35 (5.4) and 0.18 (5.7); rows off 16 bytes less: 2560 x 200 of 161 floats 0.18 (4.1) and 0.11 (3.7), 5120 x 3330 of 13
+// 0.92 (2.2) and 0.42 (2.8), which wait for the issue of instructions (whole runs of tokens through shared memory were slower).
 //
 // Codes are those of the exact quotient x / scale, which is formed rounded to odd: cut to 24 bits, with the last one set where something was
 // cut.  A code keeps far fewer bits, so it rounds from there as it would from the quotient itself (16-bit rows are full of quotients
@@ -503,17 +503,19 @@ namespace aeonb
             }
         }
 
-        // Where a lane finds its group: 32 / L.lanes groups in a warp.
+        // Where a lane finds its group: 32 / L.lanes groups in a warp.  LANES: L.lanes where that is known when compiled, else 0.
+        template <int LANES>
         struct spot
         {
             int  l, base, group, block_group; // lane of the group, its first lane, its number and that of the block's first one
             bool used;
             __device__ __forceinline__ explicit spot(const cache_launch& L)
             {
-                const int lane = threadIdx.x & 31, at_once = (int)L.by_lanes(32), mine = (int)L.by_lanes((uint32_t)lane);
-                base        = mine * L.lanes;
+                const int lane = threadIdx.x & 31, at_once = LANES ? 32 / LANES : (int)L.by_lanes(32);
+                const int mine = LANES ? lane / LANES : (int)L.by_lanes((uint32_t)lane);
+                base        = mine * (LANES ? LANES : L.lanes);
                 l           = lane - base;
-                used        = mine < at_once;
+                used        = LANES || mine < at_once;
                 block_group = (int)(blockIdx.x * (blockDim.x / 32)) * at_once;
                 group       = block_group + (int)(threadIdx.x / 32) * at_once + mine;
             }
@@ -526,12 +528,13 @@ namespace aeonb
         }
 
         // NC chunks a lane; NC = 0: as many as it takes, read a second time for their codes.
-        template <typename T, int CODE, int V, int NC>
+        template <typename T, int CODE, int V, int NC, int LANES>
         __global__ void __launch_bounds__(256, 4) cache_write_kernel(const cache_launch L)
         {
             typedef chunk<T, V>     C;
             const aeonb_cache_desc& d = L.d;
-            const spot              at(L);
+            const spot<LANES>       at(L);
+            const int               lanes = LANES ? LANES : L.lanes;
             const int               token = (int)L.by_heads((uint32_t)at.group), head = at.group - token * d.heads;
             for (int seq = blockIdx.y; seq < d.seqs; seq += gridDim.y)
             {
@@ -546,8 +549,8 @@ namespace aeonb
                     {
 #pragma unroll
                         for (int j = 0; j < NC; ++j)
-                            if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
-                                c[j].load(x + i, L.lanes, d.dim - i);
+                            if (const int i = C::place(j, at.l, lanes); i < d.dim)
+                                c[j].load(x + i, lanes, d.dim - i);
                     }
                 const int64_t place = there ? group_place(L, seq, token, head) : -1;
                 if (there && place < 0 && at.l == 0 && d.status)
@@ -559,17 +562,17 @@ namespace aeonb
                     {
 #pragma unroll
                         for (int j = 0; j < NC; ++j)
-                            if (C::place(j, at.l, L.lanes) < d.dim)
+                            if (C::place(j, at.l, lanes) < d.dim)
                                 m = max(m, c[j].largest());
                     }
                     else
-                        for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
+                        for (int j = 0, i; (i = C::place(j, at.l, lanes)) < d.dim; ++j)
                         {
-                            c[0].load(x + i, L.lanes, d.dim - i);
+                            c[0].load(x + i, lanes, d.dim - i);
                             m = max(m, c[0].largest());
                         }
                 }
-                m                 = group_largest(m, L.lanes, at.base, at.l);
+                m                 = group_largest(m, lanes, at.base, at.l);
                 const bool finite = m < INF_BITS;
                 if (__any_sync(0xffffffffu, !finite))
                 {
@@ -585,16 +588,16 @@ namespace aeonb
                         {
 #pragma unroll
                             for (int j = 0; j < NC; ++j)
-                                if (C::place(j, at.l, L.lanes) < d.dim)
+                                if (C::place(j, at.l, lanes) < d.dim)
 #pragma unroll
                                     for (int i = 0; i < C::N; ++i)
                                         see(c[j].value(i));
                         }
                         else
-                            for (int i = at.l; i < d.dim; i += L.lanes)
+                            for (int i = at.l; i < d.dim; i += lanes)
                                 see(to_float(x[i]));
                     }
-                    m = group_largest(n, L.lanes, at.base, at.l);
+                    m = group_largest(n, lanes, at.base, at.l);
                 }
                 if (place < 0)
                     continue;
@@ -608,32 +611,33 @@ namespace aeonb
                 const auto put   = [&](C& x, int i) {
                     code_words<V> q;
                     encode_chunk<T, CODE, V>(x, q, by, finite, tame, d.values != nullptr);
-                    q.store(codes + i, L.lanes, d.dim - i);
+                    q.store(codes + i, lanes, d.dim - i);
                     if (d.values)
-                        x.store(v + i, L.lanes, d.dim - i);
+                        x.store(v + i, lanes, d.dim - i);
                 };
                 if constexpr (NC > 0)
                 {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
-                        if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                        if (const int i = C::place(j, at.l, lanes); i < d.dim)
                             put(c[j], i);
                 }
                 else
-                    for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
+                    for (int j = 0, i; (i = C::place(j, at.l, lanes)) < d.dim; ++j)
                     {
-                        c[0].load(x + i, L.lanes, d.dim - i);
+                        c[0].load(x + i, lanes, d.dim - i);
                         put(c[0], i);
                     }
             }
         }
 
-        template <typename T, int CODE, int V, int NC>
+        template <typename T, int CODE, int V, int NC, int LANES>
         __global__ void __launch_bounds__(256) cache_read_kernel(const cache_launch L)
         {
             typedef chunk<T, V>     C;
             const aeonb_cache_desc& d = L.d;
-            const spot              at(L);
+            const spot<LANES>       at(L);
+            const int               lanes = LANES ? LANES : L.lanes;
             if (!at.used || at.group >= L.groups)
                 return;
             const int token = (int)L.by_heads((uint32_t)at.group), head = at.group - token * d.heads;
@@ -658,8 +662,8 @@ namespace aeonb
                     {
 #pragma unroll
                         for (int j = 0; j < NC; ++j)
-                            if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
-                                q[j].load(codes + i, L.lanes, d.dim - i);
+                            if (const int i = C::place(j, at.l, lanes); i < d.dim)
+                                q[j].load(codes + i, lanes, d.dim - i);
                     }
                 }
                 const auto put = [&](const code_words<V>& q, int i) {
@@ -668,20 +672,20 @@ namespace aeonb
                         c.fill(scale);
                     else
                         decode_chunk<T, CODE, V>(c, q, scale);
-                    c.store(v + i, L.lanes, d.dim - i);
+                    c.store(v + i, lanes, d.dim - i);
                 };
                 if constexpr (NC > 0)
                 {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
-                        if (const int i = C::place(j, at.l, L.lanes); i < d.dim)
+                        if (const int i = C::place(j, at.l, lanes); i < d.dim)
                             put(q[j], i);
                 }
                 else
-                    for (int j = 0, i; (i = C::place(j, at.l, L.lanes)) < d.dim; ++j)
+                    for (int j = 0, i; (i = C::place(j, at.l, lanes)) < d.dim; ++j)
                     {
                         if (place >= 0)
-                            q[0].load(codes + i, L.lanes, d.dim - i);
+                            q[0].load(codes + i, lanes, d.dim - i);
                         put(q[0], i);
                     }
             }
@@ -737,42 +741,59 @@ namespace aeonb
                 throw std::invalid_argument("negative stride");
         }
 
-        template <typename T, int CODE, int V, int NC>
+        template <typename T, int CODE, int V, int NC, int LANES = 0>
         void launch_lanes(cache_launch& L, bool write, cudaStream_t stream)
         {
             const int chunks  = (L.d.dim + chunk<T, V>::N - 1) / chunk<T, V>::N;
-            L.lanes           = NC ? (chunks + NC - 1) / NC : 32;
+            L.lanes           = LANES ? LANES : NC ? (chunks + NC - 1) / NC : 32;
             L.by_lanes        = fast_divisor(L.lanes);
             const int at_once = 32 / L.lanes;
             const int warps   = (int)std::min<int64_t>(8, ((int64_t)L.groups + at_once - 1) / at_once);
             const int each    = warps * at_once;
             const dim3 grid((unsigned)(((int64_t)L.groups + each - 1) / each), (unsigned)std::min(L.d.seqs, 65535));
             if (write)
-                cache_write_kernel<T, CODE, V, NC><<<grid, warps * 32, 0, stream>>>(L);
+                cache_write_kernel<T, CODE, V, NC, LANES><<<grid, warps * 32, 0, stream>>>(L);
             else
-                cache_read_kernel<T, CODE, V, NC><<<grid, warps * 32, 0, stream>>>(L);
+                cache_read_kernel<T, CODE, V, NC, LANES><<<grid, warps * 32, 0, stream>>>(L);
+        }
+
+        // Values apart: lanes known when compiled, so that a lane's values lie at fixed distances, and few slots without a value.  2560 x 200
+        // groups of 161 floats, lanes known when run / when compiled: written in 0.24 / 0.18 ms, read in 0.13 / 0.11; 64 x 1024 of 4100
+        // bf16 written in 0.65 / 0.47.
+        template <typename T, int CODE>
+        void launch_apart(cache_launch& L, bool write, cudaStream_t stream)
+        {
+            const int dim = L.d.dim;
+            if (dim <= 2 * 8)
+                launch_lanes<T, CODE, APART, 2, 2>(L, write, stream);
+            else if (dim <= 4 * 8)
+                launch_lanes<T, CODE, APART, 2, 4>(L, write, stream);
+            else if (dim <= 8 * 8)
+                launch_lanes<T, CODE, APART, 2, 8>(L, write, stream);
+            else if (dim <= 8 * 12)
+                launch_lanes<T, CODE, APART, 3, 8>(L, write, stream);
+            else if (dim <= 16 * 8)
+                launch_lanes<T, CODE, APART, 2, 16>(L, write, stream);
+            else if (dim <= 16 * 12)
+                launch_lanes<T, CODE, APART, 3, 16>(L, write, stream);
+            else if (dim <= 16 * 16)
+                launch_lanes<T, CODE, APART, 4, 16>(L, write, stream);
+            else if (dim <= 32 * 12)
+                launch_lanes<T, CODE, APART, 3, 32>(L, write, stream);
+            else
+                launch_lanes<T, CODE, APART, 0, 32>(L, write, stream);
         }
 
         template <typename T, int CODE, int V>
         void launch_chunks(cache_launch& L, bool write, cudaStream_t stream)
         {
-            const int chunks = (L.d.dim + chunk<T, V>::N - 1) / chunk<T, V>::N;
-            if (V == APART && chunks > 32 && chunks <= 32 * 3)
-            {
-                // as many chunks a lane as leave the fewest lanes without values (161 values: 14 lanes with three, two groups to a warp)
-                const auto idle = [&](int n) {
-                    const int lanes = (chunks + n - 1) / n;
-                    return lanes > 32 ? 1.0 : 1.0 - (double)(32 / lanes) * L.d.dim / (32.0 * 4 * n);
-                };
-                if (idle(3) < idle(2) && idle(3) <= idle(4))
-                    return launch_lanes<T, CODE, V, 3>(L, write, stream);
-            }
+            const int chunks = L.d.dim / V;
             // Four chunks a lane where that leaves a thousand lanes to an SM, else two: what a lane finds out about its group serves them all.
             // 64 x 4096 x 8 groups of 128 bf16 with values, two / four: to e4m3 0.24 / 0.23 ms, to int8 0.24 / 0.22, read back
             // 0.13 / 0.13; 2560 x 2000 groups of 40 floats to int8 0.37 / 0.35, read back 0.20 / 0.18; 256 x 200 of them, half there,
             // 10.3 / 12.3 us.
             const bool many = (int64_t)L.d.seqs * L.groups * chunks / 4 >= 148 * 1024;
-            if (chunks <= 32 * 2 && !(many && chunks >= 4 && V != APART))
+            if (chunks <= 32 * 2 && !(many && chunks >= 4))
                 launch_lanes<T, CODE, V, 2>(L, write, stream);
             else if (chunks <= 32 * 4)
                 launch_lanes<T, CODE, V, 4>(L, write, stream);
@@ -815,7 +836,7 @@ namespace aeonb
             {
             case 32: launch_chunks<T, CODE, 32 / sizeof(T)>(L, write, stream); break;
             case 16: launch_chunks<T, CODE, 16 / sizeof(T)>(L, write, stream); break;
-            default: launch_chunks<T, CODE, APART>(L, write, stream); break;
+            default: launch_apart<T, CODE>(L, write, stream); break;
             }
         }
 
