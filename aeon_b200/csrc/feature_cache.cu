@@ -45,20 +45,25 @@ namespace aeonb
             int              lanes;  // of a group
             int              groups; // of a sequence
             fast_divisor     by_heads, by_page, by_lanes;
+            int64_t          positions;      // that the table reaches
+            int64_t          by_page_groups; // groups of a page
         };
+
+        // a b, a not negative: two multiplications of 32 bits
+        __device__ __forceinline__ int64_t times(int a, int64_t b) { return (int64_t)((uint64_t)(uint32_t)a * (uint64_t)b); }
 
         // Where a group's codes and scale lie; -1 for a token without a place.
         __device__ __forceinline__ int64_t group_place(const cache_launch& L, int seq, int token, int head)
         {
             const aeonb_cache_desc& d  = L.d;
             const int64_t           at = (int64_t)token + (d.start ? d.start[seq] : 0);
-            if (at < 0 || at >= (int64_t)d.table_pages * d.page_tokens)
+            if (at < 0 || at >= L.positions)
                 return -1;
             const uint32_t page_of = at < 0x7fffffff ? L.by_page((uint32_t)at) : (uint32_t)at / (uint32_t)d.page_tokens; // (at is below 2^32)
-            const int32_t  page    = d.table[seq * d.table_stride + page_of];
+            const int32_t  page    = d.table[times(seq, d.table_stride) + page_of];
             if (page < 0 || page >= d.pages)
                 return -1;
-            return ((int64_t)page * d.page_tokens + ((uint32_t)at - page_of * (uint32_t)d.page_tokens)) * d.heads + head;
+            return times(page, L.by_page_groups) + times(d.heads, (uint32_t)at - page_of * (uint32_t)d.page_tokens) + head;
         }
 
         __device__ __forceinline__ int tokens_of(const aeonb_cache_desc& d, int seq)
@@ -317,15 +322,25 @@ namespace aeonb
                 }
                 else
                 {
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-                    m = max(m & 0xffffu, m >> 16);
+                    // (NaN stays; no sign, so the larger float has the larger bits)
                     if constexpr (std::is_same<T, __half>::value)
-                        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+                    {
+                        __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+                        for (int i = 1; i < W; ++i)
+                            m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+                        const float2 v = __half22float2(m);
+                        return max(__float_as_uint(v.x) & ABS_BITS, __float_as_uint(v.y) & ABS_BITS);
+                    }
                     else
-                        return m << 16;
+                    {
+                        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+                        for (int i = 1; i < W; ++i)
+                            m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+                        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&m);
+                        return max(bits << 16 & ABS_BITS, bits & 0x7fff0000u);
+                    }
                 }
             }
             __device__ __forceinline__ float value(int i) const
@@ -414,8 +429,16 @@ namespace aeonb
 
         // The largest magnitude among a group's lanes, L of them from lane `base` on (any L: the largest of some values does not
         // mind which of them it has seen twice).
+        template <int LANES>
         __device__ __forceinline__ uint32_t group_largest(uint32_t m, int L, int base, int l)
         {
+            if constexpr (LANES > 0 && LANES < 32)
+            {
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1)
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                return m;
+            }
             if (L == 32)
                 return __reduce_max_sync(0xffffffffu, m);
             for (int o = 1; o < L; o *= 2)
@@ -449,58 +472,56 @@ namespace aeonb
                 }
         }
 
-        // Codes of a chunk; with `values` the chunk then holds the values that they stand for.  finite: no -infinity in the group; tame: it
-        // has a scale, and that is so large that remainders are exact.
+        // Codes of a chunk of finite values, whose group has a scale so large that remainders are exact (or nothing but zeros); with
+        // `values` the chunk then holds the values that they stand for.
         template <typename T, int CODE, int V>
-        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, code_words<V>& q, const divisor& by, bool finite, bool tame, bool values)
+        __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, code_words<V>& q, const divisor& by, bool values)
         {
-            constexpr int N     = chunk<T, V>::N;
-            const float   scale = by.scale;
-            uint32_t      gone  = 0; // a bit for each -infinity, which counts as 0 meanwhile
-            if (!finite)
 #pragma unroll
-                for (int i = 0; i < N / 2; ++i)
-                {
-                    const float2 v = x.pair(i);
-                    const bool   a = __float_as_uint(v.x) == MINUS_INF, b = __float_as_uint(v.y) == MINUS_INF;
-                    gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
-                    x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
-                }
-            if (tame)
+            for (int i = 0; i < chunk<T, V>::N / 4; ++i)
             {
-#pragma unroll
-                for (int i = 0; i < N / 4; ++i)
+                float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
+                q.w[i] = encode4<CODE>(a, b, by);
+                if (values)
                 {
-                    float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
-                    q.w[i] = encode4<CODE>(a, b, by);
-                    if (values)
-                    {
-                        if (CODE != AEONB_CODE_INT8)
-                            numbers4<CODE>(q.w[i], a, b);
-                        x.set(2 * i, mul2(a, scale));
-                        x.set(2 * i + 1, mul2(b, scale));
-                    }
+                    if (CODE != AEONB_CODE_INT8)
+                        numbers4<CODE>(q.w[i], a, b);
+                    x.set(2 * i, mul2(a, by.scale));
+                    x.set(2 * i + 1, mul2(b, by.scale));
                 }
             }
-            else
+        }
+
+        // Any chunk: of a group with -infinities, or without a scale, or with one that small.
+        template <typename T, int CODE, int V>
+        __device__ __forceinline__ void encode_any_chunk(chunk<T, V>& x, code_words<V>& q, const divisor& by, bool tame)
+        {
+            constexpr int N    = chunk<T, V>::N;
+            uint32_t      gone = 0; // a bit for each -infinity, which counts as 0 meanwhile
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
             {
+                const float2 v = x.pair(i);
+                const bool   a = __float_as_uint(v.x) == MINUS_INF, b = __float_as_uint(v.y) == MINUS_INF;
+                gone |= (a ? 1u : 0u) << (2 * i) | (b ? 2u : 0u) << (2 * i);
+                x.set(i, make_float2(a ? 0.0f : v.x, b ? 0.0f : v.y));
+            }
+            if (tame)
+                encode_chunk<T, CODE, V>(x, q, by, false);
+            else
 #pragma unroll
                 for (int i = 0; i < N / 4; ++i)
                 {
                     const float2 a = x.pair(2 * i), b = x.pair(2 * i + 1);
-                    q.w[i] = encode_exactly<CODE>(a.x, scale) | encode_exactly<CODE>(a.y, scale) << 8 | encode_exactly<CODE>(b.x, scale) << 16 |
-                             encode_exactly<CODE>(b.y, scale) << 24;
+                    q.w[i] = encode_exactly<CODE>(a.x, by.scale) | encode_exactly<CODE>(a.y, by.scale) << 8 |
+                             encode_exactly<CODE>(b.x, by.scale) << 16 | encode_exactly<CODE>(b.y, by.scale) << 24;
                 }
-                decode_chunk<T, CODE, V>(x, q, scale);
-            }
-            if (gone && scale == scale)
-            {
+            if (by.scale == by.scale)
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (gone >> i & 1)
                         q.w[i / 4] = (q.w[i / 4] & ~(0xffu << (8 * (i & 3)))) | (CODE == AEONB_CODE_INT8 ? 0x80u : 0xffu) << (8 * (i & 3));
-                decode_chunk<T, CODE, V>(x, q, scale);
-            }
+            decode_chunk<T, CODE, V>(x, q, by.scale);
         }
 
         // Where a lane finds its group: 32 / L.lanes groups in a warp.  LANES: L.lanes where that is known when compiled, else 0.
@@ -524,7 +545,7 @@ namespace aeonb
         template <typename T>
         __device__ __forceinline__ T* group_rows(void* p, int seq, int token, int head, int64_t by_seq, int64_t by_token, int64_t by_head)
         {
-            return static_cast<T*>(p) + seq * by_seq + token * by_token + head * by_head;
+            return static_cast<T*>(p) + times(seq, by_seq) + times(token, by_token) + times(head, by_head);
         }
 
         // NC chunks a lane; NC = 0: as many as it takes, read a second time for their codes.
@@ -572,7 +593,7 @@ namespace aeonb
                             m = max(m, c[0].largest());
                         }
                 }
-                m                 = group_largest(m, lanes, at.base, at.l);
+                m                 = group_largest<LANES>(m, lanes, at.base, at.l);
                 const bool finite = m < INF_BITS;
                 if (__any_sync(0xffffffffu, !finite))
                 {
@@ -597,7 +618,7 @@ namespace aeonb
                             for (int i = at.l; i < d.dim; i += lanes)
                                 see(to_float(x[i]));
                     }
-                    m = group_largest(n, lanes, at.base, at.l);
+                    m = group_largest<LANES>(n, lanes, at.base, at.l);
                 }
                 if (place < 0)
                     continue;
@@ -606,27 +627,46 @@ namespace aeonb
                 const bool    tame = scale > 0x1p-90f || m == 0;
                 if (at.l == 0)
                     d.scales[place] = scale;
-                uint8_t*   codes = static_cast<uint8_t*>(d.codes) + place * d.dim;
+                uint8_t*   codes = static_cast<uint8_t*>(d.codes) + times(d.dim, place);
                 T*         v     = group_rows<T>(d.values, seq, token, head, d.value_stride_seq, d.value_stride_token, d.value_stride_head);
-                const auto put   = [&](C& x, int i) {
+                const auto put   = [&](C& x, int i, bool usual) {
                     code_words<V> q;
-                    encode_chunk<T, CODE, V>(x, q, by, finite, tame, d.values != nullptr);
+                    if (usual)
+                        encode_chunk<T, CODE, V>(x, q, by, d.values != nullptr);
+                    else
+                        encode_any_chunk<T, CODE, V>(x, q, by, tame);
                     q.store(codes + i, lanes, d.dim - i);
                     if (d.values)
                         x.store(v + i, lanes, d.dim - i);
                 };
-                if constexpr (NC > 0)
+                if (finite && tame)
+                {
+                    if constexpr (NC > 0)
+                    {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j)
+                            if (const int i = C::place(j, at.l, lanes); i < d.dim)
+                                put(c[j], i, true);
+                    }
+                    else
+                        for (int j = 0, i; (i = C::place(j, at.l, lanes)) < d.dim; ++j)
+                        {
+                            c[0].load(x + i, lanes, d.dim - i);
+                            put(c[0], i, true);
+                        }
+                }
+                else if constexpr (NC > 0)
                 {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
                         if (const int i = C::place(j, at.l, lanes); i < d.dim)
-                            put(c[j], i);
+                            put(c[j], i, false);
                 }
                 else
                     for (int j = 0, i; (i = C::place(j, at.l, lanes)) < d.dim; ++j)
                     {
                         c[0].load(x + i, lanes, d.dim - i);
-                        put(c[0], i);
+                        put(c[0], i, false);
                     }
             }
         }
@@ -654,7 +694,7 @@ namespace aeonb
                     if (place < 0 && at.l == 0 && d.status)
                         *d.status = 1;
                 }
-                const uint8_t* codes = static_cast<const uint8_t*>(d.codes) + place * d.dim;
+                const uint8_t* codes = static_cast<const uint8_t*>(d.codes) + times(d.dim, place);
                 if (place >= 0)
                 {
                     scale = d.scales[place];
@@ -796,7 +836,18 @@ namespace aeonb
             if (chunks <= 32 * 2 && !(many && chunks >= 4))
                 launch_lanes<T, CODE, V, 2>(L, write, stream);
             else if (chunks <= 32 * 4)
+            {
+                // (the usual sizes with the lanes known when compiled)
+                if constexpr (V * sizeof(T) == 32)
+                    switch (chunks)
+                    {
+                    case 4: return launch_lanes<T, CODE, V, 4, 1>(L, write, stream);
+                    case 8: return launch_lanes<T, CODE, V, 4, 2>(L, write, stream);
+                    case 16: return launch_lanes<T, CODE, V, 4, 4>(L, write, stream);
+                    case 32: return launch_lanes<T, CODE, V, 4, 8>(L, write, stream);
+                    }
                 launch_lanes<T, CODE, V, 4>(L, write, stream);
+            }
             else
                 launch_lanes<T, CODE, V, 0>(L, write, stream);
         }
@@ -863,6 +914,8 @@ namespace aeonb
                 L.groups   = d.tokens * d.heads;
                 L.by_heads = fast_divisor(d.heads);
                 L.by_page  = fast_divisor(d.page_tokens);
+                L.positions      = (int64_t)d.table_pages * d.page_tokens;
+                L.by_page_groups = (int64_t)d.page_tokens * d.heads;
                 const int64_t  groups = (int64_t)d.seqs * d.tokens * d.heads;
                 const int64_t  values = groups * d.dim;
                 const cudaStream_t stream = d.stream ? static_cast<cudaStream_t>(d.stream) : ctx->stream;
