@@ -879,38 +879,46 @@ namespace aeonb
                         const int have = needed ? mine.left : 0, coming = needed_then ? next.left : 0;
                         float     m    = fmaxf(one, lowest);
                         float2    z    = make_float2(pow2(__fmul_rn(__fsub_rn(one, m), L.c)), 0.0f);
+                        const auto first_pass = [&](auto all) {
+                            constexpr bool whole = decltype(all)::value;
 #pragma unroll
-                        for (int q = 0; q < CHUNKS; ++q)
-                        {
-                            wait_copies(MODE == LOSS ? CHUNKS - 1 : CHUNKS - 1 - q);
-                            if (q * CHUNK * NT < have)
+                            for (int q = 0; q < CHUNKS; ++q)
                             {
-                                piece<T> x[CHUNK];
-                                float    higher = m;
-#pragma unroll
-                                for (int i = 0; i < CHUNK; ++i)
+                                wait_copies(MODE == LOSS ? CHUNKS - 1 : CHUNKS - 1 - q);
+                                if (whole || q * CHUNK * NT < have)
                                 {
-                                    if ((q * CHUNK + i) * NT < have)
-                                        vector(x[i], q * CHUNK + i);
-                                    else
-                                        x[i].clear();
-                                    higher = x[i].largest(higher);
+                                    piece<T> x[CHUNK];
+                                    float    higher = m;
+#pragma unroll
+                                    for (int i = 0; i < CHUNK; ++i)
+                                    {
+                                        if (whole || (q * CHUNK + i) * NT < have)
+                                            vector(x[i], q * CHUNK + i);
+                                        else
+                                            x[i].clear();
+                                        higher = x[i].largest(higher);
+                                    }
+                                    const float scale = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
+                                    m                 = higher;
+                                    z                 = mul2(z, make_float2(scale, scale));
+#pragma unroll
+                                    for (int i = 0; i < CHUNK; ++i)
+                                        z = x[i].sum(z, m, L.c);
                                 }
-                                const float scale = pow2(__fmul_rn(__fsub_rn(m, higher), L.c));
-                                m                 = higher;
-                                z                 = mul2(z, make_float2(scale, scale));
+                                if (MODE == LOSS)
+                                {
 #pragma unroll
-                                for (int i = 0; i < CHUNK; ++i)
-                                    z = x[i].sum(z, m, L.c);
+                                    for (int i = 0; i < CHUNK; ++i)
+                                        fetch(s_then + next.at, coming, q * CHUNK + i);
+                                    commit();
+                                }
                             }
-                            if (MODE == LOSS)
-                            {
-#pragma unroll
-                                for (int i = 0; i < CHUNK; ++i)
-                                    fetch(s_then + next.at, coming, q * CHUNK + i);
-                                commit();
-                            }
-                        }
+                        };
+                        // The loss alone looks at none of the numbers where a thread has all its vectors.
+                        if (MODE == LOSS && have > (NV - 1) * NT)
+                            first_pass(std::true_type());
+                        else
+                            first_pass(std::false_type());
                         const float wm = warp_reduce(m, larger());
                         const float wz = warp_reduce(__fmul_rn(__fadd_rn(z.x, z.y), pow2(__fmul_rn(__fsub_rn(m, wm), L.c))), add());
                         if (lane == 0)
