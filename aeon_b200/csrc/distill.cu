@@ -15,7 +15,7 @@
 //
 // Measured on B200, 6.55 TB/s being what a copy reaches (events around a call, inputs not in L2): 8192 rows of 131072 bf16 logits with 64
 // entries: with gradient 0.84 ms (5.1 TB/s), gradient alone 0.69 (6.2), loss alone 0.46 (4.7); 65536 rows of 16384: 0.74 (5.8), 0.76
-// (5.6), 0.42 (5.1); 32768 rows of 16384 floats with gradient 0.69 (6.2); 131072 rows of 4096 bf16 0.46 (4.6), 65536 of 500 57 us (2.3).
+// (5.6), 0.40 (5.4); 32768 rows of 16384 floats with gradient 0.69 (6.2); 131072 rows of 4096 bf16 0.46 (4.6), 65536 of 500 57 us (2.3).
 // Rows of 16-bit values wait for the issue of instructions and, where a row takes several blocks, for the other blocks' sums.
 #include <algorithm>
 #include <atomic>
@@ -914,7 +914,8 @@ namespace aeonb
                                 }
                             }
                         };
-                        // The loss alone looks at none of the numbers where a thread has all its vectors.
+                        // The loss alone looks at none of the numbers where a thread has all its vectors (65536 rows of 16384 bf16: 422 us else,
+                        // now 396; with a gradient that costs the registers of a second copy: 32768 rows of 32000, 721 us as it is, 837 so).
                         if (MODE == LOSS && have > (NV - 1) * NT)
                             first_pass(std::true_type());
                         else

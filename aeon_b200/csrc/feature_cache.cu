@@ -5,9 +5,9 @@
 // that is no finite number are infinities looked at one by one.  Floor: the bytes of rows, codes and scales.
 //
 // Measured on B200, 6.55 TB/s being what a copy reaches (events around a call, inputs not in L2): 64 x 4096 x 8 groups of 128 bf16 with
-// values to e4m3 0.23 ms (5.9 TB/s), to int8 0.22 (6.2), read back 0.13 (6.3); of 64 floats 0.20 (6.1) and 0.11 (6.3); 2560 x 2000 of
-// 40 floats 0.35 (5.4) and 0.18 (5.7); rows off 16 bytes less: 2560 x 200 of 161 floats 0.18 (4.1) and 0.11 (3.7), 5120 x 3330 of 13
-// 0.92 (2.2) and 0.42 (2.8), which wait for the issue of instructions (whole runs of tokens through shared memory were slower).
+// values to e4m3 0.21 ms (6.5 TB/s), to int8 0.21 (6.5), read back 0.13 (6.3); of 64 floats 0.19 (6.5) and 0.11 (6.3); 2560 x 2000 of
+// 40 floats 0.31 (5.9) and 0.17 (6.1); rows off 16 bytes less: 2560 x 200 of 161 floats 0.16 (4.7) and 0.10 (4.0), 5120 x 3330 of 13
+// 0.91 (2.3) and 0.40 (2.9), which wait for the issue of instructions (whole runs of tokens through shared memory were slower).
 //
 // Codes are those of the exact quotient x / scale, which is formed rounded to odd: cut to 24 bits, with the last one set where something was
 // cut.  A code keeps far fewer bits, so it rounds from there as it would from the quotient itself (16-bit rows are full of quotients
