@@ -389,3 +389,62 @@ def test_random_cases_round_trip(ctx):
         rows, table = features(rng, (seqs, tokens, heads, dim), dtype), tables(rng, seqs, n, c.pages)
         start = torch.from_numpy(rng.integers(0, 5, seqs).astype(np.int32)).cuda()
         round_trip(ctx, c, rows, table, start, None, code, dtype)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("chunks", [4, 5, 8, 16, 24, 32])
+@pytest.mark.parametrize("shift", [0, 16])
+def test_large_calls_equal_small_ones(ctx, code, dtype, chunks, shift):
+    """Calls of so many groups that a lane takes four chunks of each, on 32 and on 16 bytes: the same bits as in small calls, and the
+    oracle's where groups hold infinities, NaN, nothing but zeros or the smallest numbers."""
+    rng = np.random.default_rng(chunks * 2 + shift)
+    t = TYPES[dtype]
+    size = torch.finfo(t).bits // 8
+    dim = chunks * (32 - shift) // size
+    seqs, heads, page = 37, 2, 24
+    tokens = 148 * 1024 * 4 // (chunks * seqs * heads) + 9  # lanes in all: above a thousand for each of 148 SMs
+
+    def room():
+        all_of = torch.full((seqs * tokens * heads * dim + shift,), 7.0, dtype=t, device="cuda")
+        return all_of[shift // size:][:seqs * tokens * heads * dim].view(seqs, tokens, heads, dim)
+
+    rows = room()
+    torch.manual_seed(chunks)
+    rows.copy_(torch.randn(rows.shape, device="cuda") * torch.exp2(torch.randint(-12, 12, rows.shape[:3] + (1,), device="cuda").float()))
+    special = rows[5]  # one sequence's groups
+    kinds = torch.arange(tokens, device="cuda") % 9
+    special[kinds == 0, :, 1] = float("-inf")
+    special[kinds == 1] = 0.0
+    special[kinds == 2, 0, dim - 1] = float("nan")
+    special[kinds == 3, 1, dim // 2] = float("inf")
+    special[kinds == 4] = TINY[dtype]
+    special[kinds == 5, 0] = torch.finfo(t).max
+    special[kinds == 6, 1] = float("-inf")
+    special[kinds == 7] *= torch.finfo(t).smallest_normal
+    n = (tokens + 30) // page + 1
+    big, small = cache(ctx, seqs * n, page, heads, dim, code), cache(ctx, seqs * n, page, heads, dim, code)
+    table = tables(rng, seqs, n, big.pages)
+    start = torch.from_numpy(rng.integers(0, 30, seqs).astype(np.int32)).cuda()
+    lengths = rng.integers(0, tokens + 1, seqs).astype(np.int32)
+    lengths[:7] = [0, 1, tokens, tokens, tokens, tokens, 2]
+    length = torch.from_numpy(lengths).cuda()
+    bits = {4: torch.int32, 2: torch.int16}[size]
+    values, apart = room(), room()
+    big.write(rows, table, start, length, values)
+    for s in range(seqs):
+        one = slice(s, s + 1)
+        small.write(rows[one], table[one], start[one], length[one], apart[one])
+    assert torch.equal(big.codes.view(torch.uint8), small.codes.view(torch.uint8))
+    assert torch.equal(big.scales.view(torch.int32), small.scales.view(torch.int32))
+    assert torch.equal(values.isnan(), apart.isnan())
+    assert torch.equal(values.nan_to_num(0.5).view(bits), apart.nan_to_num(0.5).view(bits))
+    out = big.read(table, tokens, start, length, out=room())
+    pieces = torch.cat([small.read(table[s:s + 1], tokens, start[s:s + 1], length[s:s + 1], dtype=t) for s in range(seqs)])
+    assert torch.equal(out.isnan(), pieces.isnan())
+    assert torch.equal(out.nan_to_num(0.5).view(bits), pieces.nan_to_num(0.5).view(bits))
+    q, s = ocache.encode(special.double().cpu().numpy(), code)
+    close(out[5], ocache.decode(q, s, code), dtype)
+    close(values[5], ocache.decode(q, s, code), dtype)
+    big.write(rows, table, start, length, rows)  # in place
+    assert torch.equal(rows[5].isnan(), out[5].isnan()) and torch.equal(rows[5].nan_to_num(0.5), out[5].nan_to_num(0.5))
