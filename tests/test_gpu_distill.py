@@ -432,3 +432,51 @@ def test_profile_counts_the_launches(ctx):
     got = ctx.profile_read()["other"]
     ctx.profile(False)
     assert got["launches"] == 2 and got["algorithmic_bytes"] == 2 * 8 * (1000 * 2 * 2 + 6 * 8 + 8)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,k", [(7001, 2100, 20), (4201, 7001, 64), (4100, 8192, 20), (2303, 16384, 20), (2200, 12001, 70), (1201, 32001, 20),
+                                          (1100, 50257, 129), (301, 131077, 64)])
+def test_rounds_of_rows(ctx, dtype, rows, vocab, k):
+    """Several rows for each block, one after the other, some of them without weight or entries: every row's result is the one that
+    it has in any other place, and that of the oracle on a sample."""
+    from aeon_b200 import kernels as K
+    rng = np.random.default_rng(rows)
+    g = torch.Generator("cuda")
+    g.manual_seed(rows)
+    wide = (vocab + 15) // 8 * 8  # whole multiples of 16 bytes: a row may change its place
+    logits = torch.randn(rows, wide, generator=g, device="cuda").mul_(3).to(TYPES[dtype])[:, 3:3 + vocab]
+    ids = torch.randint(0, vocab, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+    ids[:, k // 2] = ids[:, 0]
+    teacher = torch.randn(rows, k, generator=g, device="cuda")
+    weights = torch.rand(rows, generator=g, device="cuda") + 0.5
+    none = torch.rand(rows, generator=g, device="cuda")
+    none[rows // 2:rows // 2 + rows // 3] = 0.9  # a run of whole rounds
+    weights[none > 0.7] = 0.0
+    ids[(none > 0.5) & (none < 0.6)] = -1
+    counts = (weights != 0) & (ids >= 0).any(1)
+    up = torch.randn(rows, generator=g, device="cuda")
+    loss, lse, grad = K.distill_loss(ctx, logits, ids, teacher, 1.5, weights, up)
+    alone = K.distill_loss(ctx, logits, ids, teacher, 1.5, weights, want_grad=False)
+    grad2 = K.distill_grad(ctx, logits, ids, teacher, alone[1], 1.5, weights, up)
+    assert not loss[~counts].any() and not alone[0][~counts].any() and not grad[~counts].any() and not grad2[~counts].any()
+
+    order = torch.randperm(rows, generator=g, device="cuda")
+    other = torch.empty_strided(logits.shape, logits.stride(), dtype=logits.dtype, device="cuda")  # on 16 bytes
+    moved = torch.zeros(rows, wide, dtype=logits.dtype, device="cuda")[:, 3:3 + vocab]
+    moved.copy_(logits[order])
+    there = K.distill_loss(ctx, moved, ids[order], teacher[order], 1.5, weights[order], up[order])
+    for a, b in zip((loss, lse, grad), there):
+        assert torch.equal(a[order], b)
+    there = K.distill_loss(ctx, moved, ids[order], teacher[order], 1.5, weights[order], want_grad=False)
+    for a, b in zip(alone[:2], there[:2]):
+        assert torch.equal(a[order], b)
+    assert torch.equal(grad2[order], K.distill_grad(ctx, moved, ids[order], teacher[order], alone[1][order], 1.5, weights[order], up[order], grad=other))
+
+    at = np.unique(np.concatenate([rng.integers(0, rows, 16), [0, rows - 1]]))
+    to = torch.from_numpy(at).cuda()
+    w, u = weights[to].double().cpu().numpy(), up[to].double().cpu().numpy()
+    want = odistill.distill(logits[to].double().cpu().numpy(), ids[to].cpu().numpy(), teacher[to].double().cpu().numpy(), 1.5, w, u)
+    tol = bounds(logits[to].double().cpu().numpy(), want, dtype, 1.5, w, w * u * 1.5, k)
+    for got, i in ((loss, 0), (lse, 1), (grad, 2), (alone[0], 0), (alone[1], 1), (grad2, 2)):
+        compare(got[to], want[i], tol[i], ("loss", "lse", "gradient")[i])
