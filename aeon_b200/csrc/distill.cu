@@ -793,9 +793,9 @@ namespace aeonb
         // (and the other blocks') together, hands out what the gradient needs, and writes the entries' own part when the rest is there.
         // So the others wait once in a row, from their last exponential to the first store.  (8192 rows of 131072 bf16 logits with gradient:
         // 1.30 ms with the row in registers and all threads at every barrier, 1.22 in shared memory, 0.91 with the warp of its own.)
-        // Several blocks on an SM hide what one waits for: 3, 5, 9 or 15 by their size, at 32 to 40 registers a thread.
+        // Several blocks on an SM hide what one waits for: 3 to 15 by their size, at 32 to 40 registers a thread.
         template <typename T, int MODE, int NT, int ROOM>
-        __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : NT == 256 ? 5 : NT == 128 ? 9 : 15) distill_block_kernel(const distill_launch L)
+        __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : NT == 256 ? 5 : NT == 192 ? 7 : NT == 128 ? 9 : NT == 96 ? 12 : 15) distill_block_kernel(const distill_launch L)
         {
             constexpr int NV = BLOCK_VECTORS, CHUNK = NT == 512 ? 2 : 4, CHUNKS = NV / CHUNK, WARPS = NT / 32, N = piece<T>::N, ALL = NT + 32;
             constexpr int SUMS = 1, RESULT = 2, WRITTEN = 3; // barriers
@@ -1060,7 +1060,7 @@ namespace aeonb
                     if (MODE != GRAD)
                     {
                         bar_sync(SUMS, ALL);
-                        float2 o = lane < WARPS ? part[lane & (WARPS - 1)] : make_float2(lowest, 0.0f);
+                        float2 o = lane < WARPS ? part[min(lane, WARPS - 1)] : make_float2(lowest, 0.0f);
                         if (MODE == LOSS)
                         {
                             __syncwarp();
@@ -1389,12 +1389,20 @@ namespace aeonb
             if (L.d.k > 64)
                 return launch_blocks<T, MODE, 256, ENTRIES>(L, stream);
             // Shorter parts: fewer threads and more blocks to an SM, unless all blocks have one to themselves.  131072 rows with gradient, always
-            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.46.
+            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.46.  Between them, the next power of two / these:
+            // 65536 rows of 6000 bf16 with gradient 344 / 291 us, loss alone 219 / 205, the gradient alone 289 / 313; 32768 rows of
+            // 12000, loss alone 207 / 188, with gradient 328 / 330, the gradient alone 289 / 307.
             const bool alone = L.d.rows * blocks <= 148;
             if (L.vectors <= BLOCK_VECTORS * 64 && !alone)
                 return launch_blocks<T, MODE, 64, 64>(L, stream);
+            if constexpr (MODE != GRAD)
+                if (L.vectors <= BLOCK_VECTORS * 96 && !alone)
+                    return launch_blocks<T, MODE, 96, 64>(L, stream);
             if (L.vectors <= BLOCK_VECTORS * 128 && !alone)
                 return launch_blocks<T, MODE, 128, 64>(L, stream);
+            if constexpr (MODE == LOSS)
+                if (L.vectors <= BLOCK_VECTORS * 192 && !alone)
+                    return launch_blocks<T, MODE, 192, 64>(L, stream);
             return launch_blocks<T, MODE, 256, 64>(L, stream);
         }
 

@@ -435,7 +435,7 @@ def test_profile_counts_the_launches(ctx):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,vocab,k", [(7001, 2100, 20), (4201, 7001, 64), (4100, 8192, 20), (2303, 16384, 20), (2200, 12001, 70), (1201, 32001, 20),
+@pytest.mark.parametrize("rows,vocab,k", [(7001, 2100, 20), (4201, 7001, 64), (6001, 6000, 20), (4500, 6100, 20), (3200, 12000, 30), (4100, 8192, 20), (2303, 16384, 20), (2200, 12001, 70), (1201, 32001, 20),
                                           (1100, 50257, 129), (301, 131077, 64)])
 def test_rounds_of_rows(ctx, dtype, rows, vocab, k):
     """Several rows for each block, one after the other, some of them without weight or entries: every row's result is the one that
