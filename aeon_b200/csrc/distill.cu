@@ -430,6 +430,20 @@ namespace aeonb
             return __any_sync(0xffffffffu, twice);
         }
 
+        // The same for a short row, with a bit for each of its values.
+        __device__ __forceinline__ bool repeats_in_short_row(const int* ids, uint32_t* bits, int k, int vocab)
+        {
+            const int lane = threadIdx.x & 31;
+            for (int i = lane; i < (vocab + 31) / 32; i += 32)
+                bits[i] = 0;
+            __syncwarp();
+            bool twice = false;
+            for (int i = lane; i < k; i += 32)
+                if (const int id = ids[i]; id >= 0)
+                    twice |= (atomicOr(&bits[id / 32], 1u << (id & 31)) >> (id & 31) & 1) != 0;
+            return __any_sync(0xffffffffu, twice);
+        }
+
         __device__ __forceinline__ void write_loss(const aeonb_distill_desc& d, int64_t row, float loss, float lse)
         {
             if (d.loss)
@@ -756,7 +770,8 @@ namespace aeonb
             __syncwarp();
             if (bad)
                 return;
-            const bool twice = d.k > 32 || repeats(e.id, nullptr, d.k, 0, d.vocab);
+            // (nobody reads the entries' t any more; ids are below the vocabulary here, which is 2055 at most)
+            const bool twice = repeats_in_short_row(e.id, reinterpret_cast<uint32_t*>(e.t), d.k, d.vocab);
             for (int k = lane; k < d.k; k += 32)
             {
                 const int id = e.id[k];
@@ -1338,6 +1353,28 @@ namespace aeonb
             return cudaLaunchKernelEx(&cfg, kernel, L);
         }
 
+        // A row's part of up to 2048 vectors.  ROOM: its entries, at most.
+        template <typename T, int MODE, int ROOM>
+        cudaError_t launch_part(const distill_launch& L, cudaStream_t stream)
+        {
+            // Shorter parts: fewer threads and more blocks to an SM, unless all blocks have one to themselves.  131072 rows with gradient, always
+            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.46.  Between them, the next power of two / these:
+            // 65536 rows of 6000 bf16 with gradient 344 / 291 us, loss alone 219 / 205, the gradient alone 289 / 313; 32768 rows of
+            // 12000, loss alone 207 / 188, with gradient 328 / 330, the gradient alone 289 / 307.
+            const bool alone = L.d.rows * L.blocks <= 148;
+            if (L.vectors <= BLOCK_VECTORS * 64 && !alone)
+                return launch_blocks<T, MODE, 64, ROOM>(L, stream);
+            if constexpr (MODE != GRAD)
+                if (L.vectors <= BLOCK_VECTORS * 96 && !alone)
+                    return launch_blocks<T, MODE, 96, ROOM>(L, stream);
+            if (L.vectors <= BLOCK_VECTORS * 128 && !alone)
+                return launch_blocks<T, MODE, 128, ROOM>(L, stream);
+            if constexpr (MODE == LOSS)
+                if (L.vectors <= BLOCK_VECTORS * 192 && !alone)
+                    return launch_blocks<T, MODE, 192, ROOM>(L, stream);
+            return launch_blocks<T, MODE, 256, ROOM>(L, stream);
+        }
+
         template <typename T, int MODE>
         cudaError_t launch_mode(distill_launch& L, cudaStream_t stream)
         {
@@ -1386,24 +1423,7 @@ namespace aeonb
             if constexpr (MODE != GRAD)
                 if (L.vectors > BLOCK_VECTORS * 256)
                     return launch_blocks<T, MODE, 512, ENTRIES>(L, stream);
-            if (L.d.k > 64)
-                return launch_blocks<T, MODE, 256, ENTRIES>(L, stream);
-            // Shorter parts: fewer threads and more blocks to an SM, unless all blocks have one to themselves.  131072 rows with gradient, always
-            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.46.  Between them, the next power of two / these:
-            // 65536 rows of 6000 bf16 with gradient 344 / 291 us, loss alone 219 / 205, the gradient alone 289 / 313; 32768 rows of
-            // 12000, loss alone 207 / 188, with gradient 328 / 330, the gradient alone 289 / 307.
-            const bool alone = L.d.rows * blocks <= 148;
-            if (L.vectors <= BLOCK_VECTORS * 64 && !alone)
-                return launch_blocks<T, MODE, 64, 64>(L, stream);
-            if constexpr (MODE != GRAD)
-                if (L.vectors <= BLOCK_VECTORS * 96 && !alone)
-                    return launch_blocks<T, MODE, 96, 64>(L, stream);
-            if (L.vectors <= BLOCK_VECTORS * 128 && !alone)
-                return launch_blocks<T, MODE, 128, 64>(L, stream);
-            if constexpr (MODE == LOSS)
-                if (L.vectors <= BLOCK_VECTORS * 192 && !alone)
-                    return launch_blocks<T, MODE, 192, 64>(L, stream);
-            return launch_blocks<T, MODE, 256, 64>(L, stream);
+            return L.d.k > 64 ? launch_part<T, MODE, ENTRIES>(L, stream) : launch_part<T, MODE, 64>(L, stream);
         }
 
         template <typename T>
