@@ -14,8 +14,9 @@
 // atomics, the same bits every time.
 //
 // Measured on B200, 6.55 TB/s being what a copy reaches (events around a call, inputs not in L2): 8192 rows of 131072 bf16 logits with 64
-// entries: with gradient 0.84 ms (5.1 TB/s), gradient alone 0.69 (6.2), loss alone 0.46 (4.7); 65536 rows of 16384: 0.74 (5.8), 0.76
-// (5.6), 0.40 (5.4); 32768 rows of 16384 floats with gradient 0.69 (6.2); 131072 rows of 4096 bf16 0.46 (4.6), 65536 of 500 57 us (2.3).
+// entries: with gradient 0.84 ms (5.1 TB/s), gradient alone 0.68 (6.3), loss alone 0.45 (4.8); 65536 rows of 16384: 0.75 (5.7), 0.74
+// (5.8), 0.39 (5.5); 32768 rows of 16384 floats with gradient 0.69 (6.2); 131072 rows of 4096 bf16 0.41 (5.2), 65536 of 500 57 us (2.3);
+// with 100 entries, which one warp of a block reads, 60000 rows of 3001 0.43 (1.7).
 // Rows of 16-bit values wait for the issue of instructions and, where a row takes several blocks, for the other blocks' sums.
 #include <algorithm>
 #include <atomic>
@@ -399,11 +400,10 @@ namespace aeonb
                 grad[id] = from_float<T>(__fsub_rn(__fmul_rn(fq, pow2(__fmul_rn(__fsub_rn(s, top), L.c))), __fmul_rn(f, all)));
         }
 
-        // Whether an id in [from, to) occurs more than once among a row's entries: a warp enters them into a table of at least twice as many
-        // places.
-        constexpr int PLACES = 512;
-        static_assert(PLACES == 1 << 9 && PLACES >= 2 * ENTRIES, "the hash below has nine bits");
-        __device__ __forceinline__ bool repeats(const int* ids, int* table, int k, int from, int to)
+        // Whether an id in [from, to) occurs more than once among a row's entries: a warp compares them, or sets a bit for each in `bits`,
+        // which has room for to - from of them.  (60000 rows of 1500 floats with 100 entries each: 907 us where every entry was compared with
+        // every other one and blocks had 256 threads, 397 now.)
+        __device__ __forceinline__ bool repeats(const int* ids, uint32_t* bits, int k, int from, int to)
         {
             const int lane = threadIdx.x & 31;
             if (k <= 32)
@@ -412,35 +412,13 @@ namespace aeonb
                 const unsigned same = __match_any_sync(0xffffffffu, id); // (all lanes take part)
                 return __any_sync(0xffffffffu, id >= from && id < to && __popc(same) > 1);
             }
-            for (int i = lane; i < PLACES; i += 32)
-                table[i] = -1;
-            __syncwarp();
-            bool twice = false;
-            for (int i = lane; i < k; i += 32)
-            {
-                const int id = ids[i];
-                for (uint32_t at = (uint32_t)id * 2654435761u >> (32 - 9); id >= from && id < to; at = (at + 1) & (PLACES - 1))
-                {
-                    const int there = atomicCAS(&table[at], -1, id); // (which of two equal ones enters does not matter)
-                    twice |= there == id;
-                    if (there == -1 || there == id)
-                        break;
-                }
-            }
-            return __any_sync(0xffffffffu, twice);
-        }
-
-        // The same for a short row, with a bit for each of its values.
-        __device__ __forceinline__ bool repeats_in_short_row(const int* ids, uint32_t* bits, int k, int vocab)
-        {
-            const int lane = threadIdx.x & 31;
-            for (int i = lane; i < (vocab + 31) / 32; i += 32)
+            for (int i = lane; i < (to - from + 31) / 32; i += 32)
                 bits[i] = 0;
             __syncwarp();
             bool twice = false;
             for (int i = lane; i < k; i += 32)
-                if (const int id = ids[i]; id >= 0)
-                    twice |= (atomicOr(&bits[id / 32], 1u << (id & 31)) >> (id & 31) & 1) != 0;
+                if (const int id = ids[i]; id >= from && id < to)
+                    twice |= (atomicOr(&bits[(id - from) / 32], 1u << ((id - from) & 31)) >> ((id - from) & 31) & 1) != 0;
             return __any_sync(0xffffffffu, twice);
         }
 
@@ -771,7 +749,7 @@ namespace aeonb
             if (bad)
                 return;
             // (nobody reads the entries' t any more; ids are below the vocabulary here, which is 2055 at most)
-            const bool twice = repeats_in_short_row(e.id, reinterpret_cast<uint32_t*>(e.t), d.k, d.vocab);
+            const bool twice = repeats(e.id, reinterpret_cast<uint32_t*>(e.t), d.k, 0, d.vocab);
             for (int k = lane; k < d.k; k += 32)
             {
                 const int id = e.id[k];
@@ -820,11 +798,12 @@ namespace aeonb
                 int   found;   // 0: the row counts for nothing, the gradient is 0
                 int   ahead;   // whether the row that is copied next is needed
             };
-            extern __shared__ __align__(16) unsigned char dynamic[]; // NV x NT vectors
+            // NV x NT vectors, on the 128 bytes that a copied line fills (131072 rows of 8192 bf16 with gradient: 905 us at another place, 757 there)
+            extern __shared__ __align__(128) unsigned char row_part[];
             __shared__ float2   part[WARPS], theirs[2][16];
             __shared__ entries<ROOM> of_row[2]; // of this row and of the next one
             __shared__ outcome  result;
-            __shared__ int      table[PLACES];
+            __shared__ uint32_t ids_seen[(NV * NT * N + 2 * N + 31) / 32]; // a bit for each value of this block's part
             __shared__ uint64_t arrived[2];
             const aeonb_distill_desc& d    = L.d;
             const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -849,7 +828,7 @@ namespace aeonb
 
             if (warp < WARPS)
             {
-                const uint32_t vectors_at = shared_address(dynamic) + tid * 16;
+                const uint32_t vectors_at = shared_address(row_part) + tid * 16;
                 // this block's part of a row
                 struct share
                 {
@@ -1143,7 +1122,7 @@ namespace aeonb
                         const cut<T> c(s, d.vocab);
                         const int    begin = min(rank * L.vectors, c.n), end = min(begin + L.vectors, c.n);
                         const int    from = first ? 0 : c.head + begin * N, to = last ? d.vocab : c.head + end * N;
-                        const bool   twice = here.found && !bad && repeats(e.id, table, d.k, from, to);
+                        const bool   twice = here.found && !bad && repeats(e.id, ids_seen, d.k, from, to);
                         bar_sync(WRITTEN, ALL);
                         if (here.found && !bad)
                             for (int k = lane; k < d.k; k += 32)
@@ -1358,7 +1337,7 @@ namespace aeonb
         cudaError_t launch_part(const distill_launch& L, cudaStream_t stream)
         {
             // Shorter parts: fewer threads and more blocks to an SM, unless all blocks have one to themselves.  131072 rows with gradient, always
-            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.46.  Between them, the next power of two / these:
+            // 256 threads / by the part's length: 8192 bf16 logits 0.96 / 0.75 ms, 4096 0.80 / 0.41.  Between them, the next power of two / these:
             // 65536 rows of 6000 bf16 with gradient 344 / 291 us, loss alone 219 / 205, the gradient alone 289 / 313; 32768 rows of
             // 12000, loss alone 207 / 188, with gradient 328 / 330, the gradient alone 289 / 307.
             const bool alone = L.d.rows * L.blocks <= 148;
