@@ -23,6 +23,7 @@ namespace aeonb
 {
     namespace
     {
+        constexpr int      MAX_DIM  = 0x7fffffff - 1023;
         constexpr uint32_t ABS_BITS = 0x7fffffffu, INF_BITS = 0x7f800000u, MINUS_INF = 0xff800000u;
 
         // Division of numbers below 2^31 by one known to the host: the upper half of a product, shifted.
@@ -738,6 +739,9 @@ namespace aeonb
                 throw std::invalid_argument("the code of a cache must be AEONB_CODE_INT8 or AEONB_CODE_E4M3");
             if (d.page_tokens <= 0 || d.heads <= 0 || d.dim <= 0 || d.pages < 0)
                 throw std::invalid_argument("a cache needs page_tokens, heads and dim above 0");
+            // lanes go through a group in steps of up to 512 values, in 32 bits: the step behind the last value has to fit as well
+            if (d.dim > MAX_DIM)
+                throw std::invalid_argument("the dim of a cache is at most 2^31 - 1024");
             if (d.seqs < 0 || d.tokens < 0 || d.table_pages < 0)
                 throw std::invalid_argument("negative number of sequences, tokens or table entries");
             if ((double)d.pages * d.page_tokens * d.heads * d.dim > 0x1p62 || (double)d.seqs * d.tokens * d.heads * d.dim > 0x1p62)

@@ -366,7 +366,7 @@ typedef struct aeonb_cache_desc
     void*   codes;          /* device: pages x page_tokens x heads x dim bytes */
     float*  scales;         /* device: pages x page_tokens x heads */
     int64_t pages;
-    int32_t page_tokens, heads, dim;
+    int32_t page_tokens, heads, dim; /* each above 0, dim at most 2^31 - 1024 */
     int32_t code;           /* aeonb_cache_code */
     /* the sequences of this call */
     const int32_t* table;   /* device: page numbers, table_pages for each sequence */

@@ -1,0 +1,32 @@
+"""Ends of the ranges that the feature cache and the distillation loss take, and what the loader's passes from the cache stand on, on a
+machine without a GPU."""
+import ctypes as C
+
+import pytest
+
+from aeon_b200 import _lib as L
+from tests.test_operator_refusals import cache_desc, fake_context
+
+LARGEST_DIM = 2 ** 31 - 1024
+
+
+@pytest.mark.parametrize("name", ["aeonb_cache_write", "aeonb_cache_read"])
+@pytest.mark.parametrize("dim", [LARGEST_DIM + 1, 2 ** 31 - 512, 2 ** 31 - 128, 2 ** 31 - 1])
+def test_groups_longer_than_lanes_can_step_through(name, dim):
+    """A lane's next place, up to 512 values on, has to fit 32 bits with a sign, or it would pass for one inside the group again."""
+    lib = L.load()
+    call = getattr(lib, name)
+    one = dict(dim=dim, heads=1, pages=1, page_tokens=1, seqs=1, tokens=1)
+    assert call(fake_context(), C.byref(cache_desc(**one))) == L.ERR_INVALID
+    assert "dim" in lib.aeonb_last_error().decode()
+    assert call(fake_context(), C.byref(cache_desc(**dict(one, dim=LARGEST_DIM, seqs=0)))) == L.OK
+
+
+def test_steps_of_the_largest_group():
+    """The place behind a group's last chunk, for every width of chunk a lane takes (values at a time, lanes of a group)."""
+    for values, lanes in ((16, 32), (8, 32), (4, 32)):
+        step = values * lanes
+        for dim in (LARGEST_DIM, LARGEST_DIM - values + 1):
+            last = (dim - 1) // values * values  # of some lane
+            assert last + step + values < 2 ** 31 and dim + values - 1 < 2 ** 31
+    assert LARGEST_DIM + 4 * 32 + 3 * 32 < 2 ** 31  # values apart: four of a lane, 32 apart
