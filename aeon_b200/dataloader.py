@@ -109,7 +109,12 @@ class _CachedPasses:
         return self.serving
 
     def close(self):
+        # reads run on the streams that were current at their calls; the pages may not go to another user of the memory before
+        # the last of them
+        import torch
+        torch.cuda.synchronize(self.ctx.device)
         self.caches.clear()
+        self.tables.clear()
         self.kept.clear()
         self.ctx.close()
 

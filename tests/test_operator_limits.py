@@ -3,6 +3,7 @@ machine without a GPU."""
 import ctypes as C
 
 import pytest
+import torch
 
 from aeon_b200 import _lib as L
 from tests.test_operator_refusals import cache_desc, fake_context
@@ -30,3 +31,27 @@ def test_steps_of_the_largest_group():
             last = (dim - 1) // values * values  # of some lane
             assert last + step + values < 2 ** 31 and dim + values - 1 < 2 ** 31
     assert LARGEST_DIM + 4 * 32 + 3 * 32 < 2 ** 31  # values apart: four of a lane, 32 apart
+
+
+def test_cached_pages_are_kept_until_their_reads_are_done(monkeypatch):
+    """close() waits for the device before it lets go of anything that a read on the caller's stream may still use."""
+    from aeon_b200.dataloader import _CachedPasses
+    done = []
+
+    class Held(dict):
+        def clear(self):
+            done.append("dropped")
+            super().clear()
+
+    class Context:
+        device = 3
+
+        def close(self):
+            done.append("closed")
+
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: done.append("waited for %d" % device))
+    passes = _CachedPasses.__new__(_CachedPasses)
+    passes.ctx, passes.caches, passes.tables, passes.kept = Context(), Held(audio=1), Held(audio=2), Held(label=[3])
+    passes.close()
+    assert done[0] == "waited for 3" and done.count("dropped") == 3 and done[-1] == "closed"
+    assert not passes.caches and not passes.tables and not passes.kept
