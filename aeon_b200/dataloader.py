@@ -13,7 +13,7 @@ aeon), or torch CUDA tensors when the config sets ``"device_output": true``.  Wi
 while they are first delivered, and the other outputs as they are; the passes after the first complete one (each started by
 ``reset()``) read them from there, with no file, upload or transform.  Every pass delivers the same values: the first one those that
 its codes stand for.  It needs ``"device_output": true``, elements that are the same in every pass (audio, label, blob, top_logits)
-in the same order (no ``shuffle_enable``), and the iteration mode ONCE.
+in the same order (no ``shuffle_enable``, no ``shuffle_manifest``), and the iteration mode ONCE.
 """
 import ctypes as C
 import json
@@ -45,6 +45,9 @@ def check_feature_cache(config):
         raise ValueError("feature_cache needs the iteration mode ONCE")
     if config.get("shuffle_enable", False):
         raise ValueError("feature_cache keeps the order of the first pass: shuffle_enable must be off")
+    if config.get("shuffle_manifest", False):
+        # every pass has another order of the blocks, and with several nodes other records
+        raise ValueError("feature_cache keeps the records and order of the first pass: shuffle_manifest must be off")
     types = [e.get("type") for e in config.get("etl", [])]
     if "audio" not in types or set(types) - {"audio", "label", "blob", "top_logits"}:
         raise ValueError("feature_cache takes audio elements, with label, blob and top_logits beside them, not %s" % ", ".join(map(str, types)))

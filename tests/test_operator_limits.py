@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from aeon_b200 import _lib as L
-from tests.test_operator_refusals import cache_desc, fake_context
+from tests.test_operator_refusals import cache_desc, fake_context, loader_config
 
 LARGEST_DIM = 2 ** 31 - 1024
 
@@ -55,3 +55,14 @@ def test_cached_pages_are_kept_until_their_reads_are_done(monkeypatch):
     passes.close()
     assert done[0] == "waited for 3" and done.count("dropped") == 3 and done[-1] == "closed"
     assert not passes.caches and not passes.tables and not passes.kept
+
+
+@pytest.mark.parametrize("changes", [dict(), dict(node_count=2, node_id=1), dict(block_size=4)])
+def test_passes_that_differ_are_not_cached(changes):
+    """shuffle_manifest deals a new order of the blocks at each reset, and each node other records: not what a first pass has kept."""
+    from aeon_b200 import DataLoader
+    from aeon_b200.dataloader import check_feature_cache
+    with pytest.raises(ValueError, match="shuffle_manifest"):
+        DataLoader(loader_config(shuffle_manifest=True, **changes))
+    assert check_feature_cache(loader_config(shuffle_manifest=False, **changes)) == "int8"
+    assert check_feature_cache(loader_config(feature_cache=None, shuffle_manifest=True, **changes)) is None
