@@ -3,7 +3,7 @@
 // A row's logits are read from memory once: the largest value and the sum of exponentials against it (to the base 2, with log2(e) / T as a
 // factor of the difference, so that rows at the ends of the type's range do not overflow), then the gradient, which is written while
 // the row is still on the chip.  Floor: the bytes of the row in, and out with the gradient.  Sums and exponentials are held in 32
-// bits; an exponential below 2^-126 of the row's largest counts as 0 (no type of the gradient keeps such a share of the sum).
+// bits, sums of a thread's thousands of terms in 64; an exponential below 2^-126 of the row's largest counts as 0 (no type of the gradient keeps such a share of the sum).
 //   * up to 128 values, or up to 256 vectors of 16 bytes, with up to 32 entries: 8, 16 or 32 lanes per row (distill_few_kernel; with
 //     more entries distill_warp_kernel, a warp per row);
 //   * longer: one to sixteen blocks of a cluster per row, persistent, the row in shared memory (distill_block_kernel);
@@ -64,13 +64,17 @@ namespace aeonb
         {
             __device__ float operator()(float a, float b) const { return __fadd_rn(a, b); }
         };
+        struct add_wide
+        {
+            __device__ double operator()(double a, double b) const { return a + b; }
+        };
         struct larger // a NaN only where both are
         {
             __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
         };
 
-        template <typename Op>
-        __device__ __forceinline__ float warp_reduce(float v, Op op)
+        template <typename V, typename Op>
+        __device__ __forceinline__ V warp_reduce(V v, Op op)
         {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1)
@@ -86,15 +90,15 @@ namespace aeonb
             return r;
         }
 
-        template <typename Op>
-        __device__ __forceinline__ float block_reduce(float v, float* shared, Op op)
+        template <typename V, typename Op>
+        __device__ __forceinline__ V block_reduce(V v, V* shared, Op op)
         {
             v = warp_reduce(v, op);
             __syncthreads();
             if ((threadIdx.x & 31) == 0)
                 shared[threadIdx.x / 32] = v;
             __syncthreads();
-            float r = shared[0];
+            V r = shared[0];
             for (int i = 1; i < (int)blockDim.x / 32; ++i)
                 r = op(r, shared[i]);
             return r;
@@ -1151,7 +1155,9 @@ namespace aeonb
         template <typename T>
         __global__ void __launch_bounds__(THREADS) distill_kernel(const distill_launch L)
         {
+            constexpr int RUN = 16;
             __shared__ float          shared[THREADS / 32];
+            __shared__ double         wide[THREADS / 32];
             __shared__ entries<ENTRIES> e;
             __shared__ float          esum2_;
             __shared__ int            flags;
@@ -1187,20 +1193,38 @@ namespace aeonb
                         grad[v] = from_float<T>(0.0f);
                 return;
             }
-            float m = -inf, z = 0.0f;
-            for (int64_t v = tid; v < d.vocab; v += THREADS)
+            // The sum against a reference, which follows the largest value once that is 2^4 times as much: an exponential is 2^4 at most,
+            // and few rescalings of a sum are of any weight.  Sixteen terms in 32 bits, then in 64: a thread may have millions.  (A row of
+            // 2^26 bf16 logits, nearly alike: the lse off by 1.4e-3 with one 32-bit sum a thread, by 1.1e-6 so.  Sixteen loads at once: 16
+            // rows of 4000001, loss alone 2.46 -> 1.76 ms.)
+            float  m = -inf, ref = -inf;
+            double total = 0.0;
+            for (int64_t v0 = tid; v0 < d.vocab; v0 += RUN * THREADS)
             {
-                const float x = to_float(s[v]);
-                if (x > m)
+                float x[RUN], higher = m;
+#pragma unroll
+                for (int i = 0; i < RUN; ++i)
                 {
-                    z = m == -inf ? z : __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, x), L.c)));
-                    m = x;
+                    const int64_t v = v0 + i * THREADS;
+                    x[i]            = v < d.vocab ? to_float(s[v]) : -inf;
+                    higher          = fmaxf(higher, x[i]); // (not NaN)
                 }
-                if (!(x == -inf)) // a NaN stays in the sum
-                    z = __fadd_rn(z, pow2(__fmul_rn(__fsub_rn(x, m), L.c)));
+                m = higher;
+                if (__fmul_rn(__fsub_rn(m, ref), L.c) > 4.0f)
+                {
+                    total = ref == -inf ? total : total * pow2(__fmul_rn(__fsub_rn(ref, m), L.c));
+                    ref   = m;
+                }
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < RUN; ++i)
+                    if (!(x[i] == -inf)) // a NaN stays in the sum
+                        z = __fadd_rn(z, pow2(__fmul_rn(__fsub_rn(x[i], ref), L.c)));
+                total += z;
             }
             const float top = block_reduce(m, shared, larger());
-            const float sum = block_reduce(m > -inf && z == z ? __fmul_rn(z, pow2(__fmul_rn(__fsub_rn(m, top), L.c))) : z, shared, add());
+            // (a thread without a value has the sum 0, or NaN)
+            const float sum = (float)block_reduce(ref == -inf ? total : total * exp2(((double)ref - top) * L.c), wide, add_wide());
             const bool  bad = (flags & 2) || !(fabsf(top) < inf) || sum != sum;
             if (tid < 32)
             {

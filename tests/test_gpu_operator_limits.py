@@ -31,3 +31,51 @@ def test_a_read_under_way_when_the_passes_close(ctx):
     torch.cuda.synchronize()
     assert torch.equal(got, x)  # add() has put the kept values into x
     del taken
+
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype,vocab,kind", [
+    (torch.bfloat16, 2 ** 24 + 3, "alike"), (torch.bfloat16, 2 ** 26, "alike"), (torch.float32, 2 ** 25 + 1, "alike"), (torch.float16, 2 ** 25, "alike"),
+    (torch.float32, 2 ** 24 + 1, "rising"), (torch.bfloat16, 2 ** 24, "rising"), (torch.float32, 600001, "holes"), (torch.float16, 2 ** 24 + 5, "holes"),
+])
+def test_sums_over_millions_of_values(ctx, dtype, vocab, kind):
+    """The log-sum-exp of rows that no cluster holds does not lose more with every value.  Its error, with u = 2^-24 and R the range of
+    the exponents: an exponential (3 R + 4) u, the additions of sixteen of them 16 u (those in 64 bits nothing), four more roundings,
+    and four of the lse itself; a sum that is rescaled (when the largest value has grown by 2^4; after six times nothing is left of
+    what 2^24 terms made) takes an exponential's error each time, (3 5 + 4) u.  The gradient takes the lse's error and an exponential's."""
+    from aeon_b200 import kernels as K
+    g = torch.Generator("cuda")
+    g.manual_seed(vocab)
+    if kind == "alike":
+        x = torch.full((1, vocab), -0.6, device="cuda")
+        x[0, 7] = 0.0
+    elif kind == "rising":
+        x = torch.linspace(-9.0, 9.0, vocab, device="cuda")[None]
+    else:
+        x = torch.randn(1, vocab, generator=g, device="cuda") * 2
+        x[0, ::3] = float("-inf")
+        x[0, :5000] = float("-inf")
+    x = x.to(dtype)
+    ids = torch.tensor([[7, vocab - 1, vocab // 2]], dtype=torch.int32, device="cuda")
+    teacher = torch.tensor([[1.0, 0.5, -1.0]], device="cuda")
+    x[0, ids[0].long()] = torch.tensor([0.0, 0.25, 0.5], dtype=dtype, device="cuda")
+    loss, lse, grad = K.distill_loss(ctx, x, ids, teacher)
+    loss2, lse2, _ = K.distill_loss(ctx, x, ids, teacher, want_grad=False)
+    assert torch.equal(loss, loss2) and torch.equal(lse, lse2)
+    y = x[0].double()
+    want = torch.logsumexp(y, 0)
+    p = torch.softmax(teacher[0].double(), 0)
+    finite = y[y > -float("inf")]
+    reach = (finite.max() - finite.min()).item()
+    e = (3 * reach + 4) * U
+    lse_tol = e + (16 + 4 + (0 if kind == "alike" else 7 * 19) + 4 * abs(want.item())) * U
+    assert abs(lse.item() - want.item()) <= lse_tol
+    want_loss = (p * (p.log() - y[ids[0].long()] + want)).sum().item()
+    assert abs(loss.item() - want_loss) <= lse_tol + 4 * U * (reach + 40)
+    q = torch.exp(y - want)
+    tol = q * ((lse_tol + e + 4 * U) * 1.1 + torch.finfo(dtype).eps / 2 * 1.01) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 + 2.0 ** -126
+    q.scatter_add_(0, ids[0].long(), -p)
+    tol.scatter_add_(0, ids[0].long(), p * (e + 11 * U + torch.finfo(dtype).eps / 2))
+    assert ((grad[0].double() - q).abs() <= tol).all()
