@@ -16,7 +16,8 @@
 // Measured on B200, 6.55 TB/s being what a copy reaches (events around a call, inputs not in L2): 8192 rows of 131072 bf16 logits with 64
 // entries: with gradient 0.84 ms (5.1 TB/s), gradient alone 0.68 (6.3), loss alone 0.45 (4.8); 65536 rows of 16384: 0.75 (5.7), 0.74
 // (5.8), 0.39 (5.5); 32768 rows of 16384 floats with gradient 0.69 (6.2); 131072 rows of 4096 bf16 0.41 (5.2), 65536 of 500 57 us (2.3);
-// with 100 entries, which one warp of a block reads, 60000 rows of 3001 0.43 (1.7).
+// with 100 entries, which one warp of a block reads, 60000 rows of 3001 0.43 (1.7).  Above 131072 values blocks have 512 threads: 4096
+// rows of 151936 with 20 entries and gradient 0.64 (3.9), 2048 of 256000 0.44 (4.7).
 // Rows of 16-bit values wait for the issue of instructions and, where a row takes several blocks, for the other blocks' sums.
 #include <algorithm>
 #include <atomic>
@@ -405,8 +406,9 @@ namespace aeonb
         }
 
         // Whether an id in [from, to) occurs more than once among a row's entries: a warp compares them, or sets a bit for each in `bits`,
-        // which has room for to - from of them.  (60000 rows of 1500 floats with 100 entries each: 907 us where every entry was compared with
-        // every other one and blocks had 256 threads, 397 now.)
+        // which has room for ROOM of them: all that are looked at (0), or a window of them at a time.  (60000 rows of 1500 floats with 100
+        // entries each: 907 us where every entry was compared with every other one and blocks had 256 threads, 397 now.)
+        template <int ROOM = 0>
         __device__ __forceinline__ bool repeats(const int* ids, uint32_t* bits, int k, int from, int to)
         {
             const int lane = threadIdx.x & 31;
@@ -416,13 +418,19 @@ namespace aeonb
                 const unsigned same = __match_any_sync(0xffffffffu, id); // (all lanes take part)
                 return __any_sync(0xffffffffu, id >= from && id < to && __popc(same) > 1);
             }
-            for (int i = lane; i < (to - from + 31) / 32; i += 32)
-                bits[i] = 0;
-            __syncwarp();
             bool twice = false;
-            for (int i = lane; i < k; i += 32)
-                if (const int id = ids[i]; id >= from && id < to)
-                    twice |= (atomicOr(&bits[(id - from) / 32], 1u << ((id - from) & 31)) >> ((id - from) & 31) & 1) != 0;
+            do
+            {
+                const int end = ROOM ? min(to, from + ROOM) : to;
+                for (int i = lane; i < (end - from + 31) / 32; i += 32)
+                    bits[i] = 0;
+                __syncwarp();
+                for (int i = lane; i < k; i += 32)
+                    if (const int id = ids[i]; id >= from && id < end)
+                        twice |= (atomicOr(&bits[(id - from) / 32], 1u << ((id - from) & 31)) >> ((id - from) & 31) & 1) != 0;
+                __syncwarp();
+                from += ROOM;
+            } while (ROOM && from < to);
             return __any_sync(0xffffffffu, twice);
         }
 
@@ -790,7 +798,8 @@ namespace aeonb
         // (and the other blocks') together, hands out what the gradient needs, and writes the entries' own part when the rest is there.
         // So the others wait once in a row, from their last exponential to the first store.  (8192 rows of 131072 bf16 logits with gradient:
         // 1.30 ms with the row in registers and all threads at every barrier, 1.22 in shared memory, 0.91 with the warp of its own.)
-        // Several blocks on an SM hide what one waits for: 3 to 15 by their size, at 32 to 40 registers a thread.
+        // Several blocks on an SM hide what one waits for: 3 to 15 by their size, at 32 to 40 registers a thread (of those with room for 256
+        // entries, whose 8 KB leave less memory, 12 or 13 blocks of 64 threads, 10 of 96, 8 of 128 and 6 of 192).
         template <typename T, int MODE, int NT, int ROOM>
         __global__ void __launch_bounds__(NT + 32, NT == 512 ? 3 : NT == 256 ? 5 : NT == 192 ? 7 : NT == 128 ? 9 : NT == 96 ? 12 : 15) distill_block_kernel(const distill_launch L)
         {
@@ -807,8 +816,14 @@ namespace aeonb
             __shared__ float2   part[WARPS], theirs[2][16];
             __shared__ entries<ROOM> of_row[2]; // of this row and of the next one
             __shared__ outcome  result;
-            __shared__ uint32_t ids_seen[(NV * NT * N + 2 * N + 31) / 32]; // a bit for each value of this block's part
+            // A bit for each value of this block's part; where 32768 of them would leave room for two blocks on an SM instead of three, for half
+            // of it at a time (with gradient, two blocks / three: 2048 rows of 256000 bf16 logits with 20 entries 480 / 443 us, with 200 of
+            // them 910 / 765; 4096 rows of 151936 with 100 entries 1.48 / 1.18 ms).
+            constexpr int VALUES = NV * NT * N + 2 * N, SEEN = VALUES > 1 << 15 ? VALUES / 2 : VALUES;
+            __shared__ uint32_t ids_seen[(SEEN + 31) / 32];
             __shared__ uint64_t arrived[2];
+            static_assert(NT != 512 || 3 * (NV * NT * 16 + sizeof(of_row) + sizeof(ids_seen) + sizeof(part) + sizeof(theirs) + 256 + 1024) <= 228 * 1024,
+                          "three blocks on an SM, each with the kilobyte that the system takes");
             const aeonb_distill_desc& d    = L.d;
             const int                 tid  = threadIdx.x, warp = tid / 32, lane = tid & 31;
             const int64_t             step = gridDim.x / (unsigned)L.blocks;
@@ -1126,7 +1141,7 @@ namespace aeonb
                         const cut<T> c(s, d.vocab);
                         const int    begin = min(rank * L.vectors, c.n), end = min(begin + L.vectors, c.n);
                         const int    from = first ? 0 : c.head + begin * N, to = last ? d.vocab : c.head + end * N;
-                        const bool   twice = here.found && !bad && repeats(e.id, ids_seen, d.k, from, to);
+                        const bool   twice = here.found && !bad && repeats<SEEN < VALUES ? SEEN : 0>(e.id, ids_seen, d.k, from, to);
                         bar_sync(WRITTEN, ALL);
                         if (here.found && !bad)
                             for (int k = lane; k < d.k; k += 32)

@@ -79,3 +79,24 @@ def test_sums_over_millions_of_values(ctx, dtype, vocab, kind):
     q.scatter_add_(0, ids[0].long(), -p)
     tol.scatter_add_(0, ids[0].long(), p * (e + 11 * U + torch.finfo(dtype).eps / 2))
     assert ((grad[0].double() - q).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("vocab,pad", [(151936, 0), (262144, 0), (262151, 1)])
+@pytest.mark.parametrize("k", [33, 100, 256])
+def test_repeated_ids_in_long_parts(ctx, dtype, vocab, pad, k):
+    """Rows whose blocks look for repeated ids in half of their part at a time: repeats in either half only, at the ends of both, in
+    all blocks, and none."""
+    from tests.test_gpu_distill import check, make
+    rng = np.random.default_rng(vocab + k)
+    logits, ids, teacher = make(rng, 6, vocab, k, dtype, pad)
+    distinct = np.stack([rng.choice(vocab, k, replace=False) for _ in range(6)]).astype(np.int32)
+    distinct[1, 1] = distinct[1, 0] = 16391
+    distinct[2, -1] = distinct[2, 3] = 16392
+    part = (vocab // 8 // 8 + 7) // 8 * 8 * 8  # values of a block, but for those in front of the first whole vector
+    for j in range(8):
+        distinct[3, 4 * j:4 * j + 4] = [part * j + 16390, part * j + 16392, part * j + 16390, part * j + 16392]
+    distinct[3] = np.minimum(distinct[3], vocab - 1)
+    distinct[4, :32] = np.repeat(np.arange(8) * part, 4)
+    ids.copy_(torch.from_numpy(distinct))
+    check(ctx, logits, ids, teacher, 1.5, dtype=dtype)
