@@ -60,6 +60,11 @@ namespace aeonb
     {
         if (!ctx->profiling)
             return;
+        // a captured launch does not run now, and events recorded in a capture hold no time
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        AEONB_CUDA(cudaStreamIsCapturing(stream, &status));
+        if (status != cudaStreamCaptureStatusNone)
+            return;
         profile_span sp{kind, nullptr, nullptr, algorithmic_bytes};
         for (cudaEvent_t* e : {&sp.begin, &sp.end})
         {

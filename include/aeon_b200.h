@@ -53,10 +53,11 @@ void* aeonb_ctx_stream(aeonb_ctx* ctx);
 int  aeonb_ctx_synchronize(aeonb_ctx* ctx);
 
 /* Per-kernel timing of a context: with the profile on, every batch call records a pair of CUDA events around its
- * kernel on the context's stream.  aeonb_ctx_profile_read waits for the stream, adds the finished launches up and
+ * kernel on the stream that it runs on.  aeonb_ctx_profile_read waits for those launches, adds them up and
  * fills one entry per kernel kind: launches, summed device time, and the algorithmic bytes of those launches (each
  * unique input byte once + each output byte once: what a bandwidth roofline divides by the time).  Switching the
- * profile on clears the totals.  Works through every path that uses the context, the provider included. */
+ * profile on clears the totals.  Works through every path that uses the context, the provider included.  A
+ * launch that goes into a CUDA graph is not timed, nor are the graph's replays. */
 enum aeonb_kernel_kind
 {
     AEONB_KERNEL_ENTROPY = 0,      /* jpeg_entropy_parallel_kernel / jpeg_entropy_kernel */

@@ -100,3 +100,35 @@ def test_repeated_ids_in_long_parts(ctx, dtype, vocab, pad, k):
     distinct[4, :32] = np.repeat(np.arange(8) * part, 4)
     ids.copy_(torch.from_numpy(distinct))
     check(ctx, logits, ids, teacher, 1.5, dtype=dtype)
+
+
+def test_the_profile_of_a_context_whose_calls_are_captured(ctx):
+    """A captured call has no time of its own: it is left out, and the launches beside it are read as ever."""
+    from aeon_b200 import kernels as K
+    g = torch.Generator("cuda")
+    g.manual_seed(6)
+    logits = torch.randn(8, 1000, generator=g, device="cuda")
+    ids = torch.randint(0, 1000, (8, 3), generator=g, device="cuda", dtype=torch.int32)
+    teacher = torch.randn(8, 3, generator=g, device="cuda")
+    rows, table = torch.randn(4, 9, 1, 40, generator=g, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")[:, None]
+    cache = K.FeatureCache.allocate(ctx, 4, 16, 1, 40)
+    torch.cuda.synchronize()
+    ctx.profile(True)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = K.distill_loss(ctx, logits, ids, teacher)
+            cache.write(rows, table)
+            read = cache.read(table, 9)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ctx.profile_read()["other"]["launches"] == 0
+        want = K.distill_loss(ctx, logits, ids, teacher)
+        again = cache.read(table, 9)
+        got = ctx.profile_read()["other"]
+        assert got["launches"] == 2 and got["ms"] > 0
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(read, again)
+    finally:
+        ctx.profile(False)
