@@ -453,8 +453,12 @@ def _distill_grad_like(logits):
     x = _distill_rows("logits", logits)
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:  # a broadcast input
         return logits.new_empty(logits.shape)
-    span = off + (x.shape[0] - 1) * x.stride(0) + x.shape[1]
-    return logits.new_empty(span).as_strided(logits.shape, logits.stride(), off)
+    rows, vocab = x.shape
+    step = x.stride(0)
+    if rows > 1 and step > 4 * vocab + 8:  # columns out of far longer rows: their memory would not be the gradient's to take
+        step = vocab + (step - vocab) % (16 // x.element_size())
+        return logits.new_empty(off + (rows - 1) * step + vocab).as_strided((rows, vocab), (step, 1), off).view(logits.shape)
+    return logits.new_empty(off + (rows - 1) * step + vocab).as_strided(logits.shape, logits.stride(), off)
 
 
 def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstream=None, grad_scale=1.0, want_grad=True, grad=None):
@@ -463,8 +467,8 @@ def distill_loss(ctx, logits, ids, teacher, temperature=1.0, weights=None, upstr
 
     logits: (..., vocab) float32, float16 or bfloat16; ids (int32, -1 = no entry) and teacher (float32): (..., k), as the
     "top_logits" etl type delivers them; weights, upstream: (...) float32.  Returns (loss, lse, grad); grad has the strides of the
-    logits, is None without want_grad, and may be given (a tensor like logits, or logits itself).  A training step goes on with
-    logits.backward(grad)."""
+    logits (closer ones where the logits' rows are less than a fourth of what they lie apart), is None without want_grad, and may be
+    given (a tensor like logits, or logits itself).  A training step goes on with logits.backward(grad)."""
     if not want_grad:
         grad = None
     elif grad is None:

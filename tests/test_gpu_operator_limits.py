@@ -132,3 +132,23 @@ def test_the_profile_of_a_context_whose_calls_are_captured(ctx):
         assert all(torch.equal(a, b) for a, b in zip(out, want)) and torch.equal(read, again)
     finally:
         ctx.profile(False)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab,row,at", [(29, 5001, 3), (300, 9000, 8), (5000, 65537, 1)])
+def test_columns_of_far_longer_rows(ctx, dtype, vocab, row, at):
+    """A student whose answers are some columns of a wide tensor: the gradient's rows lie closer, and hold the same."""
+    from aeon_b200 import kernels as K
+    from tests.test_gpu_distill import check, make
+    rng = np.random.default_rng(vocab)
+    wide, ids, teacher = make(rng, 12, row, 5, dtype)
+    logits, ids = wide[:, at:at + vocab], ids % vocab
+    before = wide.clone()
+    loss, lse, grad = check(ctx, logits, ids, teacher, 2.0, dtype=dtype)
+    assert grad.stride(0) < vocab + 8 and torch.equal(wide, before)
+    cube = K.distill_loss(ctx, logits.unflatten(0, (3, 4)), ids.view(3, 4, 5), teacher.view(3, 4, 5), 2.0)
+    assert torch.equal(cube[2].reshape(12, vocab), grad) and torch.equal(cube[0].view(-1), loss) and torch.equal(cube[1].view(-1), lse)
+    given = K.distill_loss(ctx, logits, ids, teacher, 2.0, grad=logits)[2]
+    assert given is logits and torch.equal(logits, grad)
+    wide[:, at:at + vocab] = before[:, at:at + vocab]
+    assert torch.equal(wide, before)  # nothing but the columns

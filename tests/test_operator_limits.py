@@ -66,3 +66,22 @@ def test_passes_that_differ_are_not_cached(changes):
         DataLoader(loader_config(shuffle_manifest=True, **changes))
     assert check_feature_cache(loader_config(shuffle_manifest=False, **changes)) == "int8"
     assert check_feature_cache(loader_config(feature_cache=None, shuffle_manifest=True, **changes)) is None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab,row,at", [(29, 5000, 0), (29, 5001, 3), (500, 40000, 512), (1000, 4100, 1), (29, 36, 3), (1, 64, 0)])
+def test_memory_of_a_gradient(dtype, vocab, row, at):
+    """The gradient of some columns of longer rows takes the memory of the columns, not of the rows, and lies in its 16 bytes as they do."""
+    from aeon_b200.kernels import _distill_grad_like
+    size = torch.finfo(dtype).bits // 8
+    for shape in ((64,), (4, 16), (1,)):
+        logits = torch.empty(shape + (row,), dtype=dtype)[..., at:at + vocab]
+        grad = _distill_grad_like(logits)
+        assert grad.shape == logits.shape and grad.dtype == dtype
+        assert grad.untyped_storage().nbytes() <= 5 * logits.numel() * size + 64 * 9 * size
+        assert (grad.data_ptr() - logits.data_ptr()) % 16 == 0
+        assert vocab == 1 or grad.stride(-1) == 1
+        if shape != (1,):  # (one row is at no distance from another)
+            assert (grad.stride(-2) - logits.stride(-2)) * size % 16 == 0 and grad.view(-1, vocab).stride(0) >= vocab
+            assert grad.stride() == logits.stride() or row > 4 * vocab
+        grad.fill_(1)
