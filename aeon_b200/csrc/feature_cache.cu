@@ -9,9 +9,9 @@
 // 40 floats 0.31 (5.9) and 0.17 (6.1); rows off 16 bytes less: 2560 x 200 of 161 floats 0.16 (4.7) and 0.10 (4.0), 5120 x 3330 of 13
 // 0.91 (2.3) and 0.40 (2.9), which wait for the issue of instructions (whole runs of tokens through shared memory were slower).
 //
-// Codes are those of the exact quotient x / scale, which is formed rounded to odd: cut to 24 bits, with the last one set where something was
-// cut.  A code keeps far fewer bits, so it rounds from there as it would from the quotient itself (16-bit rows are full of quotients
-// next to the middle between two codes: ratios of small numbers, but for the rounding of the scale).
+// Codes are those of the exact quotient x / scale.  That is formed to 24 bits, the last one set where it is not exact, on the quotient's own
+// side of every middle between two codes, so that it rounds as the quotient itself would (16-bit rows are full of quotients next to
+// such a middle: ratios of small numbers, but for the rounding of the scale).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -179,11 +179,14 @@ namespace aeonb
             }
         };
 
-        // -x / scale for two values, rounded to odd.  The first guess t is not above the quotient q (in magnitude), five units of its last
-        // place below it at most; the correction by its remainder, a little too large (2^-20 of those units at most), ends at q or
-        // just above and is cut, so a q of 24 bits comes out itself and another one cut (none lies that close below a float: q has a
-        // numerator and denominator of 24 bits).  The second remainder, exact again, is 0 for the former only.  (Of this sign, the
-        // steps leave a zero's sign as it should be.)
+        // -x / scale for two values, for rounding to a code.  The first guess t is not above the quotient q (in magnitude), eight units of
+        // its last place below it at most.  The correction by its remainder, a little too large (2^-17 of those units at most), ends at q
+        // or just above and is cut.  The last bit is set where the second remainder says that this is not q.
+        // Why that rounds as q does: a middle M between two codes has at most eight bits, so the product of M and the scale has at most 32,
+        // and x, unless it is that product, differs from it by 2^-32 of it or more; so q is M or at least 2^-9 units away from it, and
+        // 2^-17 units do not carry it there.  Below M it is cut to the float below at most, which is odd; at M it is exact; above M it is
+        // cut to M at least and made odd.  (Elsewhere it may end a unit above q: a quotient can lie 2^-24 units below a float.)
+        // (Of this sign, the steps leave a zero's sign as it should be.)
         __device__ __forceinline__ float2 minus_quotient2(float2 x, const divisor& by)
         {
             const float2 t = mul2(x, by.small);
@@ -473,8 +476,8 @@ namespace aeonb
                 }
         }
 
-        // Codes of a chunk of finite values, whose group has a scale so large that remainders are exact (or nothing but zeros); with
-        // `values` the chunk then holds the values that they stand for.
+        // Codes of a chunk of finite values, whose group has a scale so large that no remainder is lost below the smallest float (or nothing
+        // but zeros); with `values` the chunk then holds the values that they stand for.
         template <typename T, int CODE, int V>
         __device__ __forceinline__ void encode_chunk(chunk<T, V>& x, code_words<V>& q, const divisor& by, bool values)
         {
