@@ -505,7 +505,7 @@ void aeonb_provider::plan_records(batch_plan& B, const void* const* elems, const
         if (outputs[o].host_produced && !(outputs[o].anchor_plane && B.anchor_planes_on_device))
             B.out_host[o].assign((size_t)batch_size * outputs[o].shape.byte_size(), 0);
     for (const stage& sg : stages)
-        if (sg.kind == stage_kind::top_logits) // no entries in the records that a short batch lacks
+        if (sg.kind == stage_kind::top_logits) // no entries in the records that a short batch lacks (delivered with batch_major off: else n records)
             std::fill(B.out_host[sg.first_output].begin(), B.out_host[sg.first_output].end(), (char)-1);
 
     // Parses the headers of one JPEG stream and registers it as a decode job (sizes only; no layout yet).

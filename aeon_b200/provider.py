@@ -103,11 +103,20 @@ class Provider:
             return (self.batch_size,) + dims
         return (int(np.prod(dims)), self.batch_size)
 
+    @staticmethod
+    def _no_entries(out):
+        """Teacher's ids of new buffers: -1 (0 would be an entry) behind the last record of a short batch."""
+        for name, array in out.items():
+            if name == "teacher_ids" or name.endswith(".teacher_ids"):
+                array[...] = -1
+        return out
+
     def run_host(self, records, out=None):
-        """Process `records` (list of tuples of bytes); returns {name: numpy array} in host memory."""
+        """Process `records` (list of tuples of bytes); returns {name: numpy array} in host memory.  A batch of fewer than batch_size
+        leaves what lies behind them in `out` as it was (with batch_major; else it is written too)."""
         ptrs, sizes, keep = self._pack(records)
         if out is None:
-            out = {name: np.zeros(self._shape(dims), NP_DTYPE[dt]) for name, dims, dt, _ in self.outputs}
+            out = self._no_entries({name: np.zeros(self._shape(dims), NP_DTYPE[dt]) for name, dims, dt, _ in self.outputs})
         outs = (C.c_void_p * len(self.outputs))(*[out[name].ctypes.data for name, _, _, _ in self.outputs])
         L.check(self.lib.aeonb_provider_run(self.handle, ptrs, sizes, len(records), outs, 0))
         return out
@@ -145,8 +154,8 @@ class Provider:
         ptrs, sizes, keep = self._pack(records)
         if out is None:
             with torch.cuda.stream(self.ctx.torch_stream):
-                out = {name: torch.zeros(self._shape(dims), dtype=_TORCH_DTYPE[dt], device="cuda:%d" % self.ctx.device)
-                       for name, dims, dt, _ in self.outputs}
+                out = self._no_entries({name: torch.zeros(self._shape(dims), dtype=_TORCH_DTYPE[dt], device="cuda:%d" % self.ctx.device)
+                                        for name, dims, dt, _ in self.outputs})
             self.ctx.torch_stream.synchronize()
         outs = (C.c_void_p * len(self.outputs))(*[out[name].data_ptr() for name, _, _, _ in self.outputs])
         L.check(self.lib.aeonb_provider_run(self.handle, ptrs, sizes, len(records), outs, 1))

@@ -152,3 +152,36 @@ def test_columns_of_far_longer_rows(ctx, dtype, vocab, row, at):
     assert given is logits and torch.equal(logits, grad)
     wide[:, at:at + vocab] = before[:, at:at + vocab]
     assert torch.equal(wide, before)  # nothing but the columns
+
+
+@pytest.mark.parametrize("batch_major", [True, False])
+def test_teacher_entries_behind_a_short_batch(ctx, batch_major):
+    """Two records where five may be: no entries behind them in buffers made by the call, which the loss counts as nothing; a caller's own
+    keep what they held, but for the layout whose rows are the batch."""
+    from aeon_b200 import kernels as K
+    from aeon_b200.provider import Provider, top_logits_record
+    P, k, n = 3, 2, 5
+    prov = Provider(ctx, {"batch_size": n, "batch_major": batch_major, "etl": [{"type": "top_logits", "max_positions": P, "k": k, "name": "big"}]})
+    ids, logits = np.array([[[1, 2], [3, 0], [4, 5]], [[6, 7], [8, 9], [0, 1]]]), np.arange(12.0).reshape(2, P, k)
+    records = [(top_logits_record(i, t),) for i, t in zip(ids, logits)]
+
+    def rows(out, name, shape):
+        a = out["big.teacher_" + name]
+        a = a.cpu().numpy() if torch.is_tensor(a) else a
+        return a if batch_major else a.T.reshape((n,) + shape)
+
+    for out in (prov.run_host(records), prov.run_device(records)):
+        assert np.array_equal(rows(out, "ids", (P, k))[:2], ids) and (rows(out, "ids", (P, k))[2:] == -1).all()
+        assert np.array_equal(rows(out, "logits", (P, k))[:2], logits) and not rows(out, "logits", (P, k))[2:].any()
+        assert rows(out, "count", (1,)).ravel().tolist() == [3, 3, 0, 0, 0]
+    if batch_major:
+        student = torch.randn(n, P, 10, device="cuda")
+        loss, _, grad = K.distill_loss(ctx, student, out["big.teacher_ids"], out["big.teacher_logits"])
+        assert loss[:2].all() and not loss[2:].any() and not grad[2:].any()
+    for make in (lambda s, t: np.full(s, 77, t), lambda s, t: torch.full(s, 77, dtype={np.int32: torch.int32, np.float32: torch.float32}[t], device="cuda")):
+        own = {name: make(prov._shape(dims), np.float32 if name.endswith("logits") else np.int32) for name, dims, _, _ in prov.outputs}
+        torch.cuda.synchronize()
+        (prov.run_device if torch.is_tensor(own["big.teacher_ids"]) else prov.run_host)(records, own)
+        assert np.array_equal(rows(own, "ids", (P, k))[:2], ids)
+        assert (rows(own, "ids", (P, k))[2:] == (77 if batch_major else -1)).all()
+        assert (rows(own, "count", (1,))[2:] == (77 if batch_major else 0)).all()
