@@ -338,6 +338,8 @@ int64_t aeonb_specgram_bytes(const aeonb_specgram_desc* descs, int n, const aeon
  *         code  = x / scale to the nearest number of the code, ties to the even one (of the exact quotient)
  *         value = code * scale, rounded to the type of the rows
  *
+ *     (Where scale * Q would pass the largest float, the scale is the next smaller one.)
+ *
  *     -infinity (the logarithm of an empty mel filter) is kept as a code of its own, -128 or 0xFF, reads back as -infinity
  *     and does not count in max|x|.  A group that holds a NaN or +infinity gets the scale NaN and reads back as NaN.
  *
